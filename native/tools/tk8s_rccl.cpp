@@ -122,9 +122,8 @@ std::string stall_phase() {
   return "";
 }
 
-// RCCL's device code is one 108 MB code object (the host's unpacked copy, utils/rccl_unpack.py);
-// HIP loads it onto a device the first time one of its kernels is referenced there -- inside
-// the communicator start, ~160 ms of its ~205 ms on the MI355X (profiles/r5_thp/). Referencing
+// HIP loads RCCL's device code onto a device the first time one of its kernels is referenced there -- inside
+// the communicator start, most of it on the MI355X. Referencing
 // a kernel of it right after the runtime's start, on a thread per device, lets that load overlap
 // the unique id's creation (~26 ms) or its wait (the other ranks). A second thread per device
 // makes the rank's stream meanwhile: the device's first queue, 15-85 ms measured between the

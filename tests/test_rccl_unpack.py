@@ -187,3 +187,18 @@ def test_doctor_reports_the_huge_page_mode(tmp_path):
     f.write_text("always madvise [never]\n")
     assert transparent_huge_pages(str(f))["status"] == "WARN"
     assert transparent_huge_pages(str(tmp_path / "missing"))["status"] == "WARN"
+
+
+def test_an_operators_build_is_kept_and_anything_else_refused(monkeypatch, tmp_path, native_build):
+    """A library with device code that was built from source (here: this repository's own) is kept
+    and becomes current; the installed RCCL, or a file that is no such library, is refused."""
+    monkeypatch.setattr(ru, "OUT", tmp_path / "kept")
+    assert not ru.unpack()["ok"]
+    assert not ru.adopt(ru.installed_library())["ok"]
+    assert not ru.adopt(tmp_path / "missing")["ok"]
+    (tmp_path / "text").write_text("no library")
+    assert not ru.adopt(tmp_path / "text")["ok"]
+    assert ru.library_dir() is None
+    assert ru.adopt(Path(native_build["libtk8s"]))["ok"]
+    assert ru.library_dir() == tmp_path / "kept" and ru.unpack() == {
+        "ok": True, "path": str(tmp_path / "kept" / ru.LIB_NAME), "changed": False}

@@ -100,8 +100,8 @@ def operator_state_dirs() -> list[Path]:
 
 
 def unpacked_rccl_env(container_env: dict, merged: dict, library_dir=None) -> dict:
-    """The fabric Job's ranks ask (``TK8S_RCCL_UNPACKED=1``) for RCCL with its gfx950 device code
-    unpacked (utils/rccl_unpack.py): THIS node's copy -- checked against THIS node's ROCm -- goes
+    """The fabric Job's ranks ask (``TK8S_RCCL_UNPACKED=1``) for the operator's own
+    RCCL build (utils/rccl_unpack.py): THIS node's copy -- checked against THIS node's ROCm -- goes
     in front of the library path the rank would otherwise have (the host's own path is
     kept, and a node whose copy is stale or missing loads its installed RCCL)."""
     if container_env.get("TK8S_RCCL_UNPACKED") != "1":

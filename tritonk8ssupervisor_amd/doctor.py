@@ -57,10 +57,11 @@ def common_checks() -> list[dict]:
     from .utils.rccl_unpack import OUT, installed_library, library_dir
 
     src = installed_library()
-    if src is not None:  # the fabric check's communicator start: 0.4 s unpacked, 1.8 s installed
+    if src is not None:  # the fabric check's communicator start: ~1.8 s with the installed one
         out.append(_check("rccl device code", OK if library_dir() else WARN,
-                          f"gfx950 code unpacked once ({OUT})" if library_dir() else
-                          f"{src} inflates its 5.3 GB bundle in every rank (~1.7 s): python3 __graft_entry__.py build"))
+                          f"an RCCL built for this GPU ({OUT})" if library_dir() else
+                          f"{src} inflates every target's code in each rank (~1.7 s); build RCCL from source for this GPU "
+                          "and give it to python3 -m tritonk8ssupervisor_amd.utils.rccl_unpack"))
         out.append(transparent_huge_pages())
     return out
 

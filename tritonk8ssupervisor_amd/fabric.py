@@ -29,11 +29,11 @@ def rccl_faults(spec: str) -> str:
 
 
 def rccl_rank_env(fake: bool = False) -> tuple[list[dict], Path | None]:
-    """Environment entries for the fabric Job's rank container, and the unpacked RCCL's directory
-    (None: the installed library). Pods get an env allowlist, so RCCL's logging switches, the
+    """Environment entries for the fabric Job's rank container, and the directory of the operator's
+    own RCCL build (None: the installed library). Pods get an env allowlist, so RCCL's logging switches, the
     fail-fast knobs and the ``rccl.*`` fault points are passed on here; with real GPUs the rank
-    loads RCCL with its gfx950 device code unpacked once per host (utils/rccl_unpack.py: no
-    5.3 GB inflation in every rank's communicator start) and runs glibc's malloc on transparent
+    loads the operator's own RCCL build for this GPU where one is kept (utils/rccl_unpack.py: no
+    inflation of every target's code in its communicator start) and runs glibc's malloc on transparent
     huge pages: HIP copies RCCL's 108 MB code object several times while loading it (its stream
     read, comgr's set_data, ...), each copy into freshly faulted 4 KiB pages -- ~190 ms of a
     285 ms load was memcpy; on huge pages (the kernel's madvise mode is enough) the communicator
@@ -41,7 +41,7 @@ def rccl_rank_env(fake: bool = False) -> tuple[list[dict], Path | None]:
     and makes its stream on threads while the unique id is made (profiles/r6_rccl_prewarm/).
     Off-switches: TK8S_RCCL_UNPACKED=0, TK8S_RCCL_THP=0, TK8S_RCCL_PREWARM=0.
 
-    The unpacked copy is asked for, not named: ``TK8S_RCCL_UNPACKED=1`` makes the agent of the
+    That build is asked for, not named: ``TK8S_RCCL_UNPACKED=1`` makes the agent of the
     node that runs the rank PREPEND its own current copy to the rank's LD_LIBRARY_PATH
     (agent._container_env: the copy is checked against the ROCm of that node, and the
     library path the node's runtime passes on is kept)."""

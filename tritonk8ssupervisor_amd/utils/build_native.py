@@ -241,10 +241,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
     precompile_python()
     from .rccl_unpack import unpack
 
-    try:  # RCCL's gfx950 device code unpacked once per host (the fabric check's communicator start)
-        rccl_unpacked = unpack(verbose=verbose)
-    except Exception as e:  # noqa: BLE001 - an optional speed-up: the installed library stays usable
-        rccl_unpacked = {"ok": False, "why": str(e)}
+    rccl_unpacked = unpack()  # an operator's own RCCL build for the fabric check, if one is kept
     out = {"libtk8s": lib, "libtk8s_rccl": rlib, "native_module": nat, "topo_module": topo, "tk8s-supervise": sup,
            "tk8s-gpujail": jail, "tk8s-container": tool_path("tk8s-container"),
            "tk8s-smi": smi, "tk8s-reuse": reuse_bin, "tk8s-hsaprobe": hsa_bin, **cos,
