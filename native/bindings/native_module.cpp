@@ -34,6 +34,17 @@ DType dtype_of(const std::string& d) {
   throw std::invalid_argument("dtype must be 'float32' or 'bfloat16'");
 }
 
+tk8s::LayerType layer_type_of(int t) {
+  if (t < 0 || t > 2) throw std::invalid_argument("type must be 0 (float32), 1 (bfloat16) or 2 (float16)");
+  return static_cast<tk8s::LayerType>(t);
+}
+
+// (values, row pitch, scales, scale pitch); zeros: not asked for
+using Fp8Tuple = std::tuple<uintptr_t, size_t, uintptr_t, size_t>;
+tk8s::Fp8Matrix fp8_of(const Fp8Tuple& t) {
+  return {ptr<uint8_t>(std::get<0>(t)), std::get<1>(t), ptr<uint8_t>(std::get<2>(t)), std::get<3>(t)};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tk8s_native, m) {
@@ -138,4 +149,52 @@ PYBIND11_MODULE(_tk8s_native, m) {
         tk8s::stream_copy(ptr<void>(dst), ptr<const void>(src), nbytes, stream_of(s));
       },
       py::arg("dst"), py::arg("src"), py::arg("nbytes"), py::arg("stream") = 0);
+
+  // ---- 8-bit layer (tritonk8ssupervisor_amd/ops/fp8.py checks tensors and calls these) ----------
+  m.def(
+      "rms_norm_fp8",
+      [](uintptr_t x, size_t ldx, uintptr_t residual, size_t ldr, uintptr_t weight, uintptr_t h, size_t ldh,
+         const Fp8Tuple& q, uintptr_t y, size_t ldy, uintptr_t rstd, size_t rows, size_t cols, double eps, int type,
+         int weight_type, uintptr_t s) {
+        const tk8s::Fp8Matrix o = fp8_of(q);
+        tk8s::rms_norm_fp8({ptr<const void>(x), ldx, ptr<const void>(residual), ldr, ptr<const void>(weight),
+                            ptr<void>(h), ldh, o.values, o.ld, o.scales, o.ld_scales, ptr<void>(y), ldy,
+                            ptr<float>(rstd), rows, cols, eps},
+                           layer_type_of(type), layer_type_of(weight_type), stream_of(s));
+      },
+      py::arg("x"), py::arg("ldx"), py::arg("residual"), py::arg("ldr"), py::arg("weight"), py::arg("h"),
+      py::arg("ldh"), py::arg("q"), py::arg("y"), py::arg("ldy"), py::arg("rstd"), py::arg("rows"), py::arg("cols"),
+      py::arg("eps"), py::arg("type"), py::arg("weight_type"), py::arg("stream") = 0);
+  m.def("rms_norm_backward_workspace", &tk8s::rms_norm_backward_workspace, py::arg("rows"), py::arg("cols"));
+  m.def(
+      "rms_norm_backward",
+      [](uintptr_t dy, size_t lddy, uintptr_t h, size_t ldh, uintptr_t weight, uintptr_t rstd, uintptr_t dh,
+         size_t lddh, uintptr_t dx, size_t lddx, uintptr_t dw, uintptr_t workspace, size_t rows, size_t cols, int type,
+         int weight_type, uintptr_t s) {
+        tk8s::rms_norm_backward({ptr<const void>(dy), lddy, ptr<const void>(h), ldh, ptr<const void>(weight),
+                                 ptr<const float>(rstd), ptr<const void>(dh), lddh, ptr<void>(dx), lddx,
+                                 ptr<float>(dw), ptr<float>(workspace), rows, cols},
+                                layer_type_of(type), layer_type_of(weight_type), stream_of(s));
+      },
+      py::arg("dy"), py::arg("lddy"), py::arg("h"), py::arg("ldh"), py::arg("weight"), py::arg("rstd"), py::arg("dh"),
+      py::arg("lddh"), py::arg("dx"), py::arg("lddx"), py::arg("dw"), py::arg("workspace"), py::arg("rows"),
+      py::arg("cols"), py::arg("type"), py::arg("weight_type"), py::arg("stream") = 0);
+  m.def(
+      "fp8_quantize",
+      [](uintptr_t x, size_t ldx, size_t rows, size_t cols, int type, const Fp8Tuple& by_rows, const Fp8Tuple& by_cols,
+         const Fp8Tuple& by_tiles, uintptr_t s) {
+        tk8s::fp8_quantize({ptr<const void>(x), ldx, rows, cols, fp8_of(by_rows), fp8_of(by_cols), fp8_of(by_tiles)},
+                           layer_type_of(type), stream_of(s));
+      },
+      py::arg("x"), py::arg("ldx"), py::arg("rows"), py::arg("cols"), py::arg("type"), py::arg("by_rows"),
+      py::arg("by_cols"), py::arg("by_tiles"), py::arg("stream") = 0);
+  m.def(
+      "fp8_matmul",
+      [](const Fp8Tuple& a, const Fp8Tuple& b, bool b_tiles, uintptr_t c, size_t ldc, size_t rows, size_t cols,
+         size_t k, int out, uintptr_t s) {
+        tk8s::fp8_matmul({fp8_of(a), fp8_of(b), b_tiles, ptr<void>(c), ldc, rows, cols, k}, layer_type_of(out),
+                         stream_of(s));
+      },
+      py::arg("a"), py::arg("b"), py::arg("b_tiles"), py::arg("c"), py::arg("ldc"), py::arg("rows"), py::arg("cols"),
+      py::arg("k"), py::arg("out"), py::arg("stream") = 0);
 }

@@ -7,6 +7,10 @@
 //       md5_tree            docs/benchmarks.md:11-12, "fetches random numbers and md5 hashes them").
 //   N6  ar_fill/ar_check  — all-reduce pattern generator + max-abs-error checker.
 //   N7  stream_copy       — device copy kernel used for local and xGMI peer-pull bandwidth probes.
+//   8-bit layer           — what the matrix cores are validated with: an RMS norm with 8-bit output,
+//       rms_norm_fp8,       its gradient, rounding to e4m3 with a power-of-two scale for each block
+//       fp8_quantize,       of 128 values, and the product of two such matrices
+//       fp8_matmul          (fp8_kernels.hip, matmul_kernels.hip).
 //
 // All launchers are asynchronous on `stream` and never allocate, synchronise or free, so a
 // caller may capture them into a hipGraph.
@@ -71,5 +75,84 @@ void stream_copy(void* dst, const void* src, size_t nbytes, hipStream_t stream);
 // of GPU wall clock pass -- so a stalled queue always drains, whoever forgets to release it.
 // Everything queued behind it on `stream` waits: a hung collective or pull, made on purpose.
 void gpu_stall(hipStream_t stream, double max_s);
+
+// ---- 8-bit layer ----------------------------------------------------------------------------
+// Values are e4m3 (OCP), scales E8M0 bytes: 2^(byte - 127), 255 = NaN. Strides are in elements.
+
+enum class LayerType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+// rows x cols values in 8 bits; row r starts at values + r * ld (16-byte boundaries). Scales lie
+// block by block: that of block b (128 columns) of row r at scales[b * ld_scales + r]; for 128 x 128
+// tiles, r counts tiles of rows. values == nullptr: not asked for.
+struct Fp8Matrix {
+  uint8_t* values;
+  size_t ld;
+  uint8_t* scales;
+  size_t ld_scales;
+};
+
+// h = x + residual, rounded to the type (no residual: h = x, nothing is stored);
+// rstd = 1 / sqrt(mean(h^2) + eps); y = h * rstd * weight. q/scales: y in 8 bits with a scale for
+// each 128 columns of a row; y itself and rstd are stored where their pointers are given. Every
+// sum and y are in 64 bits and rounded once. A block that holds a NaN or an infinity is NaN.
+struct NormArgs {
+  const void* x;
+  size_t ldx;
+  const void* residual;  // or nullptr
+  size_t ldr;
+  const void* weight;
+  void* h;  // needed with a residual; may be x or residual itself
+  size_t ldh;
+  uint8_t* q;  // or nullptr
+  size_t ldq;
+  uint8_t* scales;
+  size_t lds;
+  void* y;  // or nullptr
+  size_t ldy;
+  float* rstd;  // or nullptr
+  size_t rows, cols;
+  double eps;
+};
+void rms_norm_fp8(const NormArgs& a, LayerType type, LayerType weight_type, hipStream_t stream);
+
+// Gradients of rms_norm_fp8's y through to x (and the residual, whose gradient is the same) and
+// the weight; dh, if given, is what else flows into h. dw is in 32 bits. workspace: device memory of
+// rms_norm_backward_workspace() bytes that no other call uses at the same time.
+struct NormBackwardArgs {
+  const void* dy;
+  size_t lddy;
+  const void* h;
+  size_t ldh;
+  const void* weight;
+  const float* rstd;
+  const void* dh;  // or nullptr
+  size_t lddh;
+  void* dx;
+  size_t lddx;
+  float* dw;
+  float* workspace;
+  size_t rows, cols;
+};
+size_t rms_norm_backward_workspace(size_t rows, size_t cols);
+void rms_norm_backward(const NormBackwardArgs& a, LayerType type, LayerType weight_type, hipStream_t stream);
+
+// x in 8 bits, in any of three layouts from one read: a scale for each 128 columns of a row; the
+// transpose (cols x rows) with a scale for each 128 rows of a column; a scale for each 128 x 128.
+struct QuantizeArgs {
+  const void* x;
+  size_t ldx, rows, cols;
+  Fp8Matrix rows_out, cols_out, tiles_out;
+};
+void fp8_quantize(const QuantizeArgs& a, LayerType type, hipStream_t stream);
+
+// C[m, n] = A B^T with A m x k and B n x k in 8 bits; A has a scale for each 128 columns of a row,
+// B the same or one for each 128 x 128 (b_tiles). 32-bit sums, one rounding to the type of C.
+struct MatmulArgs {
+  Fp8Matrix a, b;
+  bool b_tiles;
+  void* c;
+  size_t ldc, m, n, k;
+};
+void fp8_matmul(const MatmulArgs& a, LayerType out, hipStream_t stream);
 
 }  // namespace tk8s
