@@ -83,7 +83,9 @@ enum class LayerType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
 // rows x cols values in 8 bits; row r starts at values + r * ld (16-byte boundaries). Scales lie
 // block by block: that of block b (128 columns) of row r at scales[b * ld_scales + r]; for 128 x 128
-// tiles, r counts tiles of rows. values == nullptr: not asked for.
+// tiles, r counts tiles of rows. values == nullptr: not asked for. fp8_matmul reads scales four rows at a
+// time: they start on 4-byte boundaries, ld_scales is a multiple of 4, and the rows up to the next
+// multiple of 4 can be read (their values do not matter).
 struct Fp8Matrix {
   uint8_t* values;
   size_t ld;

@@ -187,16 +187,623 @@ __global__ __launch_bounds__(WAVES * 64) void matmul_rows_kernel(MatmulArgs a) {
   }
 }
 
+// ------------------------------------------------------------------------------------------
+// Tiles
+// ------------------------------------------------------------------------------------------
+// A step is one block of 128 k from LDS. Rows of 128 bytes lie in LDS as 8 pieces, piece p of row r at p ^ (r / 4 % 8): of the
+// 16 rows 4 j + i that a fragment's lanes read at once, 8 hit 8 different pieces, and slot_row()
+// puts the other 8 into the other banks.
+// Tile i of 64 rows holds the rows 4 j + i (j = 0..15): one dword of scales then serves four tiles,
+// a byte each (the instruction picks it), and a lane ends with 16 neighbouring columns of C.
+// The row that lies at place p of a group of 64 in LDS (and the place of row p): neighbours change places
+// in the upper 32, so that of a fragment's rows 4 j + i those with j < 8 and j >= 8 lie in different
+// halves of the 64 banks.
+__device__ __forceinline__ int slot_row(int p) { return p ^ (p / 32 % 2); }
+
+template <int OB, int OA>
+__device__ __forceinline__ f32x4 mfma_scaled(const Fragment& b, const Fragment& a, f32x4 acc, unsigned sb, unsigned sa) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, acc, 0, 0, OB, static_cast<int>(sb), OA,
+                                                          static_cast<int>(sa));
+}
+
+constexpr int kXcds = 8;   // dies with an L2 of their own; blocks go to them in turn
+constexpr int kPanel = 8;  // tiles of A that a die's neighbouring blocks share
+
+// Block -> tile: blocks b, b + 8, ... run on one die; they take neighbouring tiles, column after
+// column of panels kPanel tiles high, so that a die's running blocks share rows of both operands.
+__device__ __forceinline__ void tile_of(unsigned block, unsigned tiles_m, unsigned tiles_n, unsigned& tm, unsigned& tn) {
+  const unsigned total = tiles_m * tiles_n, die = block % kXcds, per = total / kXcds, more = total % kXcds;
+  const unsigned t = die * per + (die < more ? die : more) + block / kXcds;
+  const unsigned panel = t / (kPanel * tiles_n), first = panel * kPanel;
+  const unsigned high = tiles_m - first < kPanel ? tiles_m - first : kPanel;
+  const unsigned in_panel = t - panel * kPanel * tiles_n;
+  tm = first + in_panel % high;
+  tn = in_panel / high;
+}
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
+}
+
+// 16 (4) bytes for each lane from base + offset to LDS at `to` + 16 (4) * lane. Written as assembly
+// so that the compiler does not wait for all of them before it next reads LDS; no register is written.
+__device__ __forceinline__ void load_lds16(unsigned to, const uint8_t* base, unsigned offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds4(unsigned to, const uint8_t* base, unsigned offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
+
+// Waits until at most kLeft of this wave's loads are on their way, then for the other waves.
+template <int kLeft> __device__ __forceinline__ void wait_and_meet() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// What a wave multiplies in one step: four tiles of 16 rows of each operand and their scales.
+struct Operands {
+  Fragment b[4], a[4];
+  unsigned sb, sa;
+};
+
+// acc += a step's 64 x 64 x 128; between(0) .. between(15) are issued one by one in the shadow of the
+// matrix instructions.
+template <class F>
+__device__ __forceinline__ void multiply_step(const Operands& f, f32x4 (&acc)[4][4], F between) {
+  auto pin = [&](int i) {
+    __builtin_amdgcn_sched_barrier(0);
+    between(i);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto four = [&](auto tag) {
+    constexpr int i = decltype(tag)::value;
+    acc[i][0] = mfma_scaled<0, i>(f.b[0], f.a[i], acc[i][0], f.sb, f.sa);
+    pin(4 * i);
+    acc[i][1] = mfma_scaled<1, i>(f.b[1], f.a[i], acc[i][1], f.sb, f.sa);
+    pin(4 * i + 1);
+    acc[i][2] = mfma_scaled<2, i>(f.b[2], f.a[i], acc[i][2], f.sb, f.sa);
+    pin(4 * i + 2);
+    acc[i][3] = mfma_scaled<3, i>(f.b[3], f.a[i], acc[i][3], f.sb, f.sa);
+    pin(4 * i + 3);
+  };
+  four(std::integral_constant<int, 0>{});
+  four(std::integral_constant<int, 1>{});
+  four(std::integral_constant<int, 2>{});
+  four(std::integral_constant<int, 3>{});
+}
+
+// The same with 32-bit sums, in two halves: B widened, then A tile by tile while it is multiplied. The
+// widening multiplies the scales in, if they are near; else they are left for scaled_sums().
+__device__ __forceinline__ void widen_b(const Operands& f, unsigned scales, Wide (&wb)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) wb[j] = widen(f.b[j], scale_value(scales >> (8 * j) & 255u));
+}
+
+__device__ __forceinline__ void multiply_wide(const Operands& f, const Wide (&wb)[4], f32x4 (&acc)[4][4]) {
+  Wide wa[2];
+  wa[0] = widen(f.a[0], scale_value(f.sa & 255u));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float scale = i < 3 ? scale_value(f.sa >> (8 * i + 8) & 255u) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      acc[i][j] = multiply(wb[j], wa[i % 2], acc[i][j]);
+      if (i < 3) {  // a quarter of the next tile is widened in the shadow of these four
+#pragma unroll
+        for (int h = 2 * j; h < 2 * j + 2; ++h) {
+          wa[1 - i % 2].pair[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f.a[i + 1].word[h], scale, false);
+          wa[1 - i % 2].pair[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f.a[i + 1].word[h], scale, true);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+__device__ __forceinline__ void scaled_sums(const Operands& f, const Wide (&wb)[4], f32x4 (&acc)[4][4], int group) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const Wide wa = widen(f.a[i], 1.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 p = multiply(wb[j], wa, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[i][j][r] += scaled(p[r], f.sa >> (8 * i) & 255u, __shfl(f.sb, 4 * group + r, 64) >> (8 * j) & 255u);
+      __builtin_amdgcn_sched_barrier(0);  // one pair at a time: this way is rare, its registers are not free
+    }
+  }
+}
+
+// A block of (TM / 64) x (TN / 64) waves makes TM x TN of C, each wave 64 x 64. kStages steps of LDS go
+// round: while a step is multiplied from registers, the next one is read from LDS and the bytes
+// of the step kStages ahead are requested (straight into LDS, no registers). One barrier a step
+// says both that the next step has arrived and that the slot to be refilled has been read. What
+// bounds it is the time a request takes against kStages - 1 steps: LDS is as full of bytes on
+// their way as it can be.
+template <class O, bool kExact, int TM, int TN, int kStages>
+__global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
+  constexpr int WM = TM / 64, WN = TN / 64, kWaves = WM * WN;
+  constexpr int kRows = (TM + TN) / 8;                       // loads of 8 rows x 128 bytes in a step
+  constexpr int kLoads = (kRows + kWaves - 1) / kWaves + 1;  // by each wave, the scales' one included
+  constexpr int kScales = (TM + TN) * 128, kSlot = kScales + 512;
+  static_assert(kWaves >= 2 && kLoads <= 16 && kStages >= 3 && kStages * kSlot <= 160 * 1024, "tile shape");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * kSlot];
+  const int lane = threadIdx.x % 64, group = lane / 16, j16 = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int wm = wave / WN, wn = wave % WN;
+  const unsigned lds0 = lds_address(lds);
+  unsigned tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const size_t m0 = static_cast<size_t>(tm) * TM, n0 = static_cast<size_t>(tn) * TN;
+  const unsigned whole = static_cast<unsigned>(a.k / kScaleBlock);
+
+  // Load c of this wave: 8 of the slot's rows, A's TM, then B's TN; pitches are below 2^23, so offsets
+  // from the tile's first row fit 32 bits. Rows behind the last one are that one again.
+  const uint8_t* const abase = a.a.values + m0 * a.a.ld;
+  const uint8_t* const bbase = a.b.values + n0 * a.b.ld;
+  unsigned off[kLoads - 1];
+#pragma unroll
+  for (int c = 0; c < kLoads - 1; ++c) {
+    const int q = std::min(wave + c * kWaves, kRows - 1);  // where they do not come out even, the last ones twice
+    const int r = slot_row(8 * q + lane / 8);
+    const unsigned piece = 16u * ((lane % 8) ^ (r / 4 % 8));
+    off[c] = r < TM ? static_cast<unsigned>(std::min<size_t>(r, a.m - 1 - m0)) * static_cast<unsigned>(a.a.ld) + piece
+                    : static_cast<unsigned>(std::min<size_t>(r - TM, a.n - 1 - n0)) * static_cast<unsigned>(a.b.ld) + piece;
+  }
+  // scales: a dword a lane of A's rows (even waves) or B's (odd waves); for 128 x 128 tiles of B the
+  // dword with those of this tile in every lane
+  const uint8_t* sbase;
+  unsigned off_s;
+  if (wave % 2 == 0) {
+    sbase = a.a.scales + m0;
+    off_s = static_cast<unsigned>(std::min<size_t>(4 * lane, (a.m - 1) / 4 * 4 - m0));
+  } else if (a.b_tiles) {
+    sbase = a.b.scales + n0 / kScaleBlock / 4 * 4;
+    off_s = 4 * (lane % 2) <= (a.n - 1) / kScaleBlock / 4 * 4 - n0 / kScaleBlock / 4 * 4 ? 4 * (lane % 2) : 0;
+  } else {
+    sbase = a.b.scales + n0;
+    off_s = static_cast<unsigned>(std::min<size_t>(4 * lane, (a.n - 1) / 4 * 4 - n0));
+  }
+  const size_t s_step = wave % 2 == 0 ? a.a.ld_scales : a.b.ld_scales;
+  // Behind the last step it is read once more, into a slot nobody reads again: the counts stay true.
+  auto load = [&](unsigned step, unsigned slot, int c) {
+    const size_t b = step < whole ? step : whole - 1;
+    if (c == 0) {
+      load_lds4(lds0 + slot * kSlot + kScales + (wave % 2) * 256, sbase + b * s_step, off_s);
+    } else {
+      const int q = std::min(wave + (c - 1) * kWaves, kRows - 1);
+      load_lds16(lds0 + slot * kSlot + q * 1024, (8 * q < TM ? abase : bbase) + b * kScaleBlock, off[c - 1]);
+    }
+  };
+
+  unsigned lane_at[2][2];
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      lane_at[odd][h] = lds0 + 512u * j16 + 128u * (odd ^ (j16 / 8)) + 16u * ((4 * h + group) ^ (j16 % 8));
+  const size_t tile_n = (n0 + wn * 64) / kScaleBlock;
+  const unsigned pick = a.b_tiles ? static_cast<unsigned>(tile_n % 4) * 0x01010101u : 0x03020100u;
+  const int at_sb = 64 + (a.b_tiles ? static_cast<int>(tile_n / 4 - n0 / kScaleBlock / 4) : wn * 16 + j16);
+  auto read_scales = [&](unsigned slot, Operands& f) {
+    const unsigned* const scales = reinterpret_cast<const unsigned*>(lds + slot * kSlot + kScales);
+    f.sa = scales[wm * 16 + j16];
+    f.sb = __builtin_amdgcn_perm(0, scales[at_sb], pick);
+  };
+  auto read_piece = [&](unsigned slot, Operands& f, int c) {  // piece c of the 16: B's, then A's
+    typedef const __attribute__((address_space(3))) u32x4* lds16;
+    const int i = c / 2 % 4, h = c % 2;
+    if (c < 8) f.b[i].half[h] = *reinterpret_cast<lds16>(lane_at[i % 2][h] + (slot * kSlot + TM * 128 + wn * 8192) + i / 2 * 256);
+    else f.a[i].half[h] = *reinterpret_cast<lds16>(lane_at[i % 2][h] + (slot * kSlot + wm * 8192) + i / 2 * 256);
+  };
+  auto read_step = [&](unsigned slot, Operands& f) {
+    read_scales(slot, f);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) read_piece(slot, f, c);
+  };
+
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Operands f[2];
+
+  // A step loaded with zeros behind the end of the rows, everything waited for.
+  auto load_slowly = [&](unsigned b) {
+    for (int q = wave; q < kRows; q += kWaves) {
+      const int r = slot_row(8 * q + lane / 8);
+      const size_t k = static_cast<size_t>(b) * kScaleBlock + 16 * ((lane % 8) ^ (r / 4 % 8));
+      const uint8_t* const src = r < TM ? a.a.values + std::min(m0 + r, a.m - 1) * a.a.ld : a.b.values + std::min(n0 + r - TM, a.n - 1) * a.b.ld;
+      *reinterpret_cast<u32x4*>(lds + q * 1024 + lane * 16) = load16(src, k, a.k);
+    }
+    load_lds4(lds0 + kScales + (wave % 2) * 256, sbase + b * s_step, off_s);
+    wait_and_meet<0>();
+  };
+
+  auto store = [&](const f32x4 (&sums)[4][4]) {
+    // lane: row 4 * j16 + i, columns 16 * group + 4 r + j
+    const size_t mw = m0 + wm * 64, col = n0 + wn * 64 + 16 * group;
+    const int left = col < a.n ? static_cast<int>(std::min<size_t>(a.n - col, 16)) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const size_t row = mw + 4 * j16 + i;
+      if (row >= a.m) continue;
+      O* const c = static_cast<O*>(a.c) + row * a.ldc + col;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = sums[i][e % 4][2 * h + e / 4];
+        store8(c + 8 * h, left - 8 * h, v);
+      }
+    }
+  };
+
+  if constexpr (!kExact) {
+    if (a.k % kScaleBlock) {  // first the block that the end of the rows cuts off
+      load_slowly(whole);
+      read_step(0, f[0]);
+      multiply_step(f[0], acc, [](int) {});
+      wait_and_meet<0>();
+    }
+    if (whole) {
+#pragma unroll
+      for (int s = 0; s < kStages; ++s)
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) load(s, s, c);
+      unsigned slot = 0;
+      wait_and_meet<(kStages - 1) * kLoads>();
+      read_step(0, f[0]);
+      auto step = [&](unsigned b, const Operands& now, Operands& then) {
+        wait_and_meet<(kStages - 2) * kLoads>();  // step b is in everyone's registers, step b + 1 in LDS
+        const unsigned next = slot + 1 == kStages ? 0 : slot + 1;
+        read_scales(next, then);
+        multiply_step(now, acc, [&](int c) {
+          read_piece(next, then, c);
+          if (c < kLoads) load(b + kStages, slot, c);
+        });
+        slot = next;
+      };
+      for (unsigned b = 0; b < whole; b += 2) {
+        step(b, f[0], f[1]);
+        if (b + 1 < whole) step(b + 1, f[1], f[0]);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may still be on its way to LDS when the block ends
+    }
+  } else {
+    // Two groups of waves take turns, one phase apart: while one reads a step and widens B, the other
+    // multiplies. A slot is refilled when the later group has read it. All waves look at all scales
+    // of a step, so they give up together when one is far and make the tile again the slow way.
+    static_assert(kStages == 3 && kWaves == 8, "two groups");
+    auto all_near = [&](unsigned slot) {
+      const unsigned* const scales = reinterpret_cast<const unsigned*>(lds + slot * kSlot + kScales);
+      const unsigned va = scales[lane % (TM / 4)], vb = scales[64 + (a.b_tiles ? lane % 2 : lane % (TN / 4))];
+      bool far = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) far = far || far_scale(va >> (8 * i) & 255u) || far_scale(vb >> (8 * i) & 255u);
+      return __builtin_amdgcn_ballot_w64(far) == 0;
+    };
+    bool near = true;
+    if (a.k % kScaleBlock) {
+      Wide wb[4];
+      load_slowly(whole);
+      read_step(0, f[0]);
+      near = all_near(0);
+      widen_b(f[0], f[0].sb, wb);
+      multiply_wide(f[0], wb, acc);
+      wait_and_meet<0>();
+    }
+    if (whole && near) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) load(s, s, c);
+      unsigned slot = 0;
+      wait_and_meet<0>();
+      if (wave >= kWaves / 2) wait_and_meet<0>();
+      for (unsigned b = 0; b < whole; ++b) {
+        near = all_near(slot);
+        if (!near) break;
+        Wide wb[4];
+        const unsigned before = slot == 0 ? kStages - 1 : slot - 1;
+        // changed as far as the compiler knows: it would otherwise keep every address of the loop in a
+        // register of its own, and sums in scratch memory
+        asm volatile("" : "+v"(lane_at[0][0]), "+v"(lane_at[0][1]), "+v"(lane_at[1][0]), "+v"(lane_at[1][1]));
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) load(b + 2, before, c);
+        read_scales(slot, f[0]);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) read_piece(slot, f[0], c);
+        __builtin_amdgcn_sched_barrier(0);
+        widen_b(f[0], f[0].sb, wb);
+        wait_and_meet<kLoads>();  // the next step is in LDS
+        multiply_wide(f[0], wb, acc);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        slot = slot + 1 == kStages ? 0 : slot + 1;
+      }
+      if (wave < kWaves / 2) wait_and_meet<0>();
+      wait_and_meet<0>();
+    }
+    if (!near) {
+      f32x4 sums[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sums[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (unsigned b = 0; b * static_cast<size_t>(kScaleBlock) < a.k; ++b) {
+        Wide wb[4];
+        load_slowly(b);
+        read_step(0, f[0]);
+        widen_b(f[0], 0x7f7f7f7fu, wb);
+        scaled_sums(f[0], wb, sums, group);
+        wait_and_meet<0>();
+      }
+      store(sums);
+      return;
+    }
+  }
+  store(acc);
+}
+
+// ------------------------------------------------------------------------------------------
+// Large tiles: 256 x 256 of C, eight waves in two groups that take turns
+// ------------------------------------------------------------------------------------------
+// Four waves (one on each SIMD unit) make the upper 128 rows, four the lower ones, each 128 x 64. A
+// step of 128 k is four phases, a barrier after each: read B and half of A from LDS | 16 matrix
+// instructions | read the other half of A | 16 matrix instructions. The lower group runs one phase
+// behind, so on every SIMD one wave multiplies while the other reads.
+// LDS holds two steps. A slot is refilled once both groups have read it -- B and the first half of A in
+// the second multiplying phase of a step, the second half in the first one of the next -- and waits
+// count the loads that may still be on their way instead of draining them: a step's bytes have
+// about four phases to arrive. Every wave issues the same nine loads a step between its matrix
+// instructions (256 bytes of scales, four pieces of 1 KiB of B, two of A's first half; two of A's
+// second half), which makes the counts the same for all.
+// LDS: two slots each of B's 256 rows, of A's first and of its second halves (128 rows each) and of the
+// scales, so that both slots lie within the reach of one address.
+constexpr int kBigB = 0, kBigA = 2 * 256 * 128, kBigHalf = 128 * 128, kBigScales = 2 * 512 * 128;
+constexpr int kBigLds = kBigScales + 2 * 512;
+
+// End of a reading phase: what this wave read has arrived, of its loads at most kLeft are on their way.
+template <int kLeft> __device__ __forceinline__ void read_end() {
+  static_assert(kLeft == 0 || kLeft == 2 || kLeft == 7, "waits");
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (kLeft == 7) asm volatile("s_waitcnt vmcnt(7) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  else if constexpr (kLeft == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// End of a multiplying phase (or a phase a group sits out).
+__device__ __forceinline__ void phase_end() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <class O>
+__global__ __launch_bounds__(512, 2) void matmul_big_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBigLds];
+  const int lane = threadIdx.x % 64, group = lane / 16, j16 = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int wm = wave / 4, wn = wave % 4;
+  const unsigned lds0 = lds_address(lds);
+
+  unsigned tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const size_t m0 = static_cast<size_t>(tm) * 256, n0 = static_cast<size_t>(tn) * 256;
+  const unsigned whole = static_cast<unsigned>(a.k / kScaleBlock);  // 1 at least
+
+  // A lane loads 16 bytes at row r of each 64 rows (pitches below 2^23: the offsets from the tile's
+  // first row fit 32 bits); rows behind the last one are that one again. Slots hold of A the rows
+  // 0-63 and 128-191 (first halves), 64-127 and 192-255 (second halves).
+  const unsigned r = static_cast<unsigned>(slot_row(8 * wave + lane / 8));
+  const unsigned piece = 16u * ((lane % 8) ^ (r / 4 % 8));
+  const unsigned lda = static_cast<unsigned>(a.a.ld), ldb = static_cast<unsigned>(a.b.ld);
+  unsigned row_a = r * lda, row_b = r * ldb;
+  const unsigned last_a = static_cast<unsigned>(std::min<size_t>(255, a.m - 1 - m0)) * lda;
+  const unsigned last_b = static_cast<unsigned>(std::min<size_t>(255, a.n - 1 - n0)) * ldb;
+  const uint8_t* const abase = a.a.values + m0 * a.a.ld;
+  const uint8_t* const bbase = a.b.values + n0 * a.b.ld;
+  // scales: the tile's 256 rows of A (even waves load them) or of B (odd waves), a dword a lane; for
+  // 128 x 128 tiles of B the dword that holds the two of this tile, in every lane
+  const uint8_t* sbase;
+  unsigned off_s;
+  if (wave % 2 == 0) {
+    sbase = a.a.scales + m0;
+    off_s = static_cast<unsigned>(std::min<size_t>(4 * lane, (a.m - 1) / 4 * 4 - m0));
+  } else if (a.b_tiles) {
+    sbase = a.b.scales + n0 / kScaleBlock / 4 * 4;
+    off_s = 0;
+  } else {
+    sbase = a.b.scales + n0;
+    off_s = static_cast<unsigned>(std::min<size_t>(4 * lane, (a.n - 1) / 4 * 4 - n0));
+  }
+  const size_t s_step = wave % 2 == 0 ? a.a.ld_scales : a.b.ld_scales;
+
+  // Load c of the nine of step b: 0 the scales, 1-4 B, 5-6 A's first halves; 7-8 its second halves.
+  // Behind the last step it is read once more, into a slot nobody reads again: the counts stay true.
+  auto load = [&](unsigned step, int c, int slot) {
+    const size_t b = step < whole ? step : whole - 1;
+    if (c == 0) load_lds4(lds0 + kBigScales + slot * 512 + (wave % 2) * 256, sbase + b * s_step, off_s);
+    else if (c < 5)
+      load_lds16(lds0 + kBigB + slot * 32768 + (wave + 8 * (c - 1)) * 1024, bbase + b * kScaleBlock,
+                 std::min(row_b + (c - 1) * 64 * ldb, last_b) + piece);
+    else
+      load_lds16(lds0 + kBigA + (2 * ((c - 5) / 2) + slot) * kBigHalf + (wave + 8 * ((c - 5) % 2)) * 1024,
+                 abase + b * kScaleBlock, std::min(row_a + ((c - 5) % 2 * 128 + (c - 5) / 2 * 64) * lda, last_a) + piece);
+  };
+
+  f32x4 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Fragment fb[4], fa[4];
+  unsigned sa[2], sb = 0;
+  sa[0] = sa[1] = 0;
+
+  // Where in 64 rows of LDS this lane finds its two pieces of an even and of an odd tile's row: all
+  // other offsets are constants of the read instructions.
+  unsigned lane_at[2][2];
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      lane_at[odd][h] = lds0 + 512u * j16 + 128u * (odd ^ (j16 / 8)) + 16u * ((4 * h + group) ^ (j16 % 8));
+  auto fragment = [&](unsigned offset, int i, int fixed) {
+    typedef const __attribute__((address_space(3))) u32x4* lds16;
+    Fragment f;
+    f.half[0] = *reinterpret_cast<lds16>(lane_at[i % 2][0] + offset + (fixed + i / 2 * 256));
+    f.half[1] = *reinterpret_cast<lds16>(lane_at[i % 2][1] + offset + (fixed + i / 2 * 256));
+    return f;
+  };
+  // 16 matrix instructions; issue(i) after each four of them, in their shadow.
+  auto multiply_half = [&](auto half, auto issue) {
+    constexpr int g = decltype(half)::value;
+    auto four = [&](auto tag) {
+      constexpr int i = decltype(tag)::value;
+      f32x4(&c)[4] = acc[g * 4 + i];
+      c[0] = mfma_scaled<0, i>(fb[0], fa[i], c[0], sb, sa[g]);
+      c[1] = mfma_scaled<1, i>(fb[1], fa[i], c[1], sb, sa[g]);
+      c[2] = mfma_scaled<2, i>(fb[2], fa[i], c[2], sb, sa[g]);
+      c[3] = mfma_scaled<3, i>(fb[3], fa[i], c[3], sb, sa[g]);
+      __builtin_amdgcn_sched_barrier(0);
+      issue(i);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    four(std::integral_constant<int, 0>{});
+    four(std::integral_constant<int, 1>{});
+    four(std::integral_constant<int, 2>{});
+    four(std::integral_constant<int, 3>{});
+  };
+  constexpr auto kHalf0 = std::integral_constant<int, 0>{};
+  constexpr auto kHalf1 = std::integral_constant<int, 1>{};
+  const auto nothing = [](int) {};
+
+  const unsigned pick = a.b_tiles ? static_cast<unsigned>((n0 / kScaleBlock + wn / 2) % 4) * 0x01010101u : 0x03020100u;
+  const int at_sb = 64 + (a.b_tiles ? 0 : wn * 16 + j16);
+  // B, the first two of this wave's four tiles in A's first half, the scales; then the other two
+  auto read_first = [&](int slot) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fb[j] = fragment(kBigB + wn * 8192, j, slot * 32768);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) fa[i] = fragment(kBigA + wm * 8192, i, slot * kBigHalf);
+    const unsigned* const scales = reinterpret_cast<const unsigned*>(lds + kBigScales + slot * 512);
+    sa[0] = scales[wm * 32 + j16];
+    sa[1] = scales[wm * 32 + 16 + j16];
+    sb = __builtin_amdgcn_perm(0, scales[at_sb], pick);
+  };
+  auto read_more = [&](int slot) {
+#pragma unroll
+    for (int i = 2; i < 4; ++i) fa[i] = fragment(kBigA + wm * 8192, i, slot * kBigHalf);
+  };
+  auto read_second = [&](int slot) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fa[i] = fragment(kBigA + wm * 8192, i, (2 + slot) * kBigHalf);
+  };
+
+  if (a.k % kScaleBlock) {  // first the block that the end of the rows cuts off, zeros behind it
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) {
+      const int row = static_cast<int>(r) + (c < 4 ? 64 * c : (c - 4) % 2 * 128 + (c - 4) / 2 * 64);
+      const uint8_t* const src = c < 4 ? a.b.values + std::min(n0 + row, a.n - 1) * a.b.ld : a.a.values + std::min(m0 + row, a.m - 1) * a.a.ld;
+      uint8_t* const to = lds + (c < 4 ? kBigB + c * 8192 : kBigA + (c - 4) / 2 * 2 * kBigHalf + (c - 4) % 2 * 8192) + wave * 1024 + lane * 16;
+      *reinterpret_cast<u32x4*>(to) = load16(src, static_cast<size_t>(whole) * kScaleBlock + piece, a.k);
+    }
+    load_lds4(lds0 + kBigScales + (wave % 2) * 256, sbase + whole * s_step, off_s);
+    read_end<0>();
+    read_first(0);
+    read_more(0);
+    multiply_half(kHalf0, nothing);
+    read_second(0);
+    multiply_half(kHalf1, nothing);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int c = 0; c < 9; ++c) load(0, c, 0);
+#pragma unroll
+  for (int c = 0; c < 7; ++c) load(1, c, 1);
+  read_end<0>();
+  if (wm == 1) phase_end();  // the lower group runs one phase behind
+  auto step = [&](unsigned b, auto parity) {
+    constexpr int slot = decltype(parity)::value;
+    // changed as far as the compiler knows: it would otherwise keep every offset of the loop, and the
+    // sums that belong in these registers in scratch memory
+    asm volatile("" : "+v"(row_a), "+v"(row_b), "+v"(lane_at[0][0]), "+v"(lane_at[0][1]), "+v"(lane_at[1][0]), "+v"(lane_at[1][1]));
+    read_first(slot);
+    read_end<7>();  // this step's second halves, requested a step ago, are there
+    read_more(slot);
+    multiply_half(kHalf0, [&](int i) { if (i < 2) load(b + 1, 7 + i, 1 - slot); });
+    phase_end();
+    read_second(slot);
+    read_end<2>();  // the next step's first seven are there
+    multiply_half(kHalf1, [&](int i) { load(b + 2, 2 * i, slot); if (i < 3) load(b + 2, 2 * i + 1, slot); });
+    phase_end();
+  };
+  for (unsigned b = 0; b + 1 < whole; b += 2) {
+    step(b, kHalf0);
+    step(b + 1, kHalf1);
+  }
+  if (whole % 2) step(whole - 1, kHalf0);
+  if (wm == 0) phase_end();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may still be on its way to LDS when the block ends
+  const size_t mw = m0 + wm * 128, col = n0 + wn * 64 + 16 * group;
+  const int left = col < a.n ? static_cast<int>(std::min<size_t>(a.n - col, 16)) : 0;
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const size_t row = mw + 64 * g + 4 * j16 + i;
+      if (row >= a.m) continue;
+      O* const c = static_cast<O*>(a.c) + row * a.ldc + col;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[g * 4 + i][e % 4][2 * h + e / 4];
+        store8(c + 8 * h, left - 8 * h, v);
+      }
+    }
+}
+
 void check(bool ok, const char* what) {
   if (!ok) throw std::invalid_argument(what);
 }
 
+template <class O, bool kExact, int TM, int TN, int kStages> void launch_stage(const MatmulArgs& a, hipStream_t stream) {
+  const size_t tm = (a.m + TM - 1) / TM, tn = (a.n + TN - 1) / TN;
+  hipLaunchKernelGGL((matmul_stage_kernel<O, kExact, TM, TN, kStages>), dim3(static_cast<unsigned>(tm * tn)), dim3(TM / 64 * (TN / 64) * 64),
+                     0, stream, a, static_cast<unsigned>(tm), static_cast<unsigned>(tn));
+}
+
 template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t stream) {
-  const unsigned gx = static_cast<unsigned>((a.n + 15) / 16);
-  if (a.m <= 16)
-    hipLaunchKernelGGL((matmul_rows_kernel<O, kExact, 1, 8, 4>), dim3(gx, 1), dim3(512), 0, stream, a);
-  else
-    hipLaunchKernelGGL((matmul_rows_kernel<O, kExact, 2, 8, 2>), dim3(gx, static_cast<unsigned>((a.m + 31) / 32)), dim3(512), 0, stream, a);
+  const bool tiled = a.m > 32 && a.a.ld < (1u << 23) && a.b.ld < (1u << 23);
+  if (!tiled) {
+    const unsigned gx = static_cast<unsigned>((a.n + 15) / 16);
+    if (a.m <= 16) hipLaunchKernelGGL((matmul_rows_kernel<O, kExact, 1, 8, 4>), dim3(gx, 1), dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((matmul_rows_kernel<O, kExact, 2, 8, 2>), dim3(gx, static_cast<unsigned>((a.m + 31) / 32)), dim3(512), 0, stream, a);
+    return;
+  }
+  const size_t big_m = (a.m + 255) / 256, big_n = (a.n + 255) / 256;
+  if constexpr (!kExact) {
+    if (big_m * big_n >= 192 && a.k >= kScaleBlock) {
+      hipLaunchKernelGGL(matmul_big_kernel<O>, dim3(static_cast<unsigned>(big_m * big_n)), dim3(512), 0, stream, a,
+                         static_cast<unsigned>(big_m), static_cast<unsigned>(big_n));
+      return;
+    }
+  }
+  if constexpr (kExact) {
+    launch_stage<O, true, 256, 128, 3>(a, stream);
+  } else {
+    if (a.m <= 64) launch_stage<O, false, 64, 128, 4>(a, stream);
+    else launch_stage<O, false, 128, 128, 4>(a, stream);
+  }
 }
 
 }  // namespace
@@ -209,9 +816,10 @@ void fp8_matmul(const MatmulArgs& a, LayerType out, hipStream_t stream) {
             a.a.ld % 16 == 0 && a.b.ld % 16 == 0,
         "fp8: the rows of 8-bit values must start on 16-byte boundaries");
   check(reinterpret_cast<uintptr_t>(a.a.scales) % 4 == 0 && a.a.ld_scales % 4 == 0 &&
-            (a.b_tiles || (reinterpret_cast<uintptr_t>(a.b.scales) % 4 == 0 && a.b.ld_scales % 4 == 0)),
+            reinterpret_cast<uintptr_t>(a.b.scales) % 4 == 0 && a.b.ld_scales % 4 == 0,
         "fp8: the scales of a block must start on a 4-byte boundary");
-  check(a.m <= (1u << 20) && a.n <= (1u << 24), "fp8_matmul: at most 2^20 rows and 2^24 columns of C");
+  check(a.m <= (1u << 20) && a.n <= (1u << 24) && (a.m + 63) / 64 * ((a.n + 63) / 64) <= (size_t(1) << 24),
+        "fp8_matmul: at most 2^20 rows and 2^24 columns of C, and 2^36 values");
   switch (out) {
     case LayerType::kF32: launch<float, true>(a, stream); break;
     case LayerType::kBF16: launch<__bf16, false>(a, stream); break;

@@ -301,6 +301,17 @@ def test_matmul_matches_the_oracle(fp8, m, n, k, tiles, out):
     check_product(fp8.matmul(a, b, dtype=out), a64, b64, k)
 
 
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("m,n,k", [(3621, 3700, 128), (3600, 3585, 300), (3585, 3612, 640), (3584, 3584, 1029)])
+def test_matmul_of_many_tiles_matches_the_oracle(fp8, m, n, k, tiles):
+    """Enough of C for the largest tiles, cut off at every side; 1 to 8 blocks of k."""
+    a, a64 = operand(fp8, m + k, m, k)
+    b, b64 = operand(fp8, n + 2 * k, n, k, tiles=tiles)
+    out = torch.full((m + 1, n + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    check_product(fp8.matmul(a, b, out=out[:m, 3:3 + n]), a64, b64, k)
+    assert (out[m:] == 7).all() and (out[:, :3] == 7).all() and (out[:, 3 + n:] == 7).all()
+
+
 def test_matmul_of_whole_numbers_is_exact(fp8):
     """Small whole numbers: every product and sum is a 32-bit value, so nothing may be off."""
     rng = np.random.default_rng(5)
