@@ -58,9 +58,11 @@ def operand(fp8, seed, rows, cols, tiles=False, spread=1.0):
     q[(q & 0x7F) == 0x7F] = 0x3A
     sr, nb = (-(-rows // 128) if tiles else rows), -(-cols // 128)
     s = rng.integers(118, 134, size=(sr, nb)).astype(np.uint8)
-    out, _ = fp8._empty(rows, cols, sr, torch.device("cuda"))
-    out.values.copy_(torch.from_numpy(q).view(torch.float8_e4m3fn))
-    out.scales.copy_(torch.from_numpy(s).view(torch.float8_e8m0fnu))
+    values = torch.empty(rows, -(-cols // 16) * 16, dtype=torch.uint8, device="cuda")[:, :cols]
+    scales = torch.empty(nb, -(-sr // 16) * 16, dtype=torch.uint8, device="cuda").t()[:sr]
+    values.copy_(torch.from_numpy(q))
+    scales.copy_(torch.from_numpy(s))
+    out = fp8.Quantized(values.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu))
     return out, ref.fp8_dequantize(q, s)
 
 

@@ -33,6 +33,13 @@ def native() -> ModuleType:
     return _load("_tk8s_native")
 
 
+def layer() -> ModuleType:
+    """The 8-bit layer on torch tensors (``ops.fp8`` documents its calls); imports PyTorch."""
+    import torch  # noqa: F401  (the module links its libraries)
+
+    return _load("_tk8s_layer")
+
+
 def topo() -> ModuleType:
     """CPU-only topology allocator (no HIP dependency)."""
     return _load("_tk8s_topo")

@@ -27,12 +27,18 @@ from typing import NamedTuple
 
 import torch
 
-from . import native
+from . import layer
 
-BLOCK = 128
+_LAYOUTS = {"rows": 0, "columns": 1, "both": 2, "tiles": 3}
+_native = None
 
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_NONE = (0, 0, 0, 0)
+
+def _layer():
+    """The module that checks the arguments, allocates and launches (native/bindings/layer_module.cpp)."""
+    global _native
+    if _native is None:
+        _native = layer()
+    return _native
 
 
 class Quantized(NamedTuple):
@@ -58,110 +64,16 @@ class Normed(NamedTuple):
         return Quantized(self.values, self.scales)
 
 
-def _up(n: int, to: int) -> int:
-    return -(-n // to) * to
-
-
-def _matrix(t, name: str) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor, not {type(t).__name__}")
-    if t.dim() != 2:
-        raise ValueError(f"{name} must have 2 dimensions, not {t.dim()}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"the rows of {name} must be contiguous (stride {t.stride(1)} between columns)")
-    return t
-
-
-def _typed(t, name: str) -> int:
-    _matrix(t, name)
-    code = _TYPES.get(t.dtype)
-    if code is None:
-        raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
-    return code
-
-
-def _like(t, name: str, x: torch.Tensor, of: str) -> torch.Tensor:
-    _matrix(t, name)
-    if t.dtype != x.dtype or t.shape != x.shape:
-        raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype} like {of}, not {tuple(t.shape)} {t.dtype}")
-    return t
-
-
-def _vector(t, name: str, size: int, dtypes: tuple) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor, not {type(t).__name__}")
-    if t.shape != (size,) or t.dtype not in dtypes or (size > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be {size} contiguous values of {' or '.join(map(str, dtypes))}, "
-                         f"not {tuple(t.shape)} {t.dtype}")
-    return t
-
-
-def _writable(t: torch.Tensor, name: str) -> torch.Tensor:
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"the rows of {name} overlap: it cannot be written to")
-    return t
-
-
-class _Device:
-    """The tensors' one GPU made current, and its stream."""
-
-    __slots__ = ("index", "before", "stream")
-
-    def __init__(self, *tensors):
-        first = tensors[0].device
-        if first.type != "cuda":
-            raise ValueError(f"the 8-bit layer runs on a GPU; the tensors are on {first}")
-        for t in tensors:
-            if t is not None and t.device != first:
-                raise ValueError(f"all tensors must be on one GPU, not on {first} and {t.device}")
-        self.index = first.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        self.stream = torch.cuda.current_stream(self.index).cuda_stream
-        return self
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-
-
-def _empty(rows: int, cols: int, scale_rows: int, device) -> tuple[Quantized, tuple]:
-    """Room for rows x cols values in 8 bits and their scales, as the kernels lay them out."""
-    ld, blocks, lds = _up(cols, 16), _up(cols, BLOCK) // BLOCK, _up(scale_rows, 16)
-    values = torch.empty((rows, ld), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty((blocks, lds), dtype=torch.float8_e8m0fnu, device=device)
-    at = (values.data_ptr(), ld, scales.data_ptr(), lds)
-    if ld != cols:
-        values = values[:, :cols]
-    return Quantized(values, scales.t()[:scale_rows]), at
-
-
 def quantize(x: torch.Tensor, *, layout: str = "rows"):
     """``x`` (rows x cols; float32, bfloat16 or float16) in 8 bits, a :class:`Quantized`.
 
     ``layout``: ``"rows"`` -- a scale for each 128 columns of a row; ``"columns"`` -- the transpose, cols
     x rows, with a scale for each 128 rows of x; ``"both"`` -- these two, as a pair, from one read;
     ``"tiles"`` -- a scale for each 128 x 128."""
-    if layout not in ("rows", "columns", "both", "tiles"):
+    if layout not in _LAYOUTS:
         raise ValueError(f"layout must be 'rows', 'columns', 'both' or 'tiles', not {layout!r}")
-    code = _typed(x, "x")
-    rows, cols = x.shape
-    with _Device(x) as dev:
-        by_rows = by_cols = by_tiles = None
-        row_at = col_at = tile_at = _NONE
-        if layout in ("rows", "both"):
-            by_rows, row_at = _empty(rows, cols, rows, x.device)
-        if layout in ("columns", "both"):
-            by_cols, col_at = _empty(cols, rows, cols, x.device)
-        if layout == "tiles":
-            by_tiles, tile_at = _empty(rows, cols, _up(rows, BLOCK) // BLOCK, x.device)
-        native().fp8_quantize(x.data_ptr(), x.stride(0), rows, cols, code, row_at, col_at, tile_at, dev.stream)
-    if layout == "both":
-        return by_rows, by_cols
-    return by_rows or by_cols or by_tiles
+    out = (_native or _layer()).quantize(x, _LAYOUTS[layout])
+    return Quantized(*out) if len(out) == 2 else (Quantized(*out[:2]), Quantized(*out[2:]))
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None, eps: float = 1e-6,
@@ -172,27 +84,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | 
 
     ``x``, ``residual``: rows x cols; float32, bfloat16 or float16. ``weight``: cols, of x's type or
     float32."""
-    code = _typed(x, "x")
-    rows, cols = x.shape
-    if residual is not None:
-        _like(residual, "residual", x, "x")
-    _vector(weight, "weight", cols, (x.dtype, torch.float32))
-    eps = float(eps)
-    if not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, but is {eps}")
-    with _Device(x, weight, residual) as dev:
-        h, ldr, ldh = x, 0, 0
-        if residual is not None:
-            h = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-            ldr, ldh = residual.stride(0), cols
-        out, at = _empty(rows, cols, rows, x.device) if quantized else (Quantized(None, None), _NONE)
-        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if normed else None
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-        native().rms_norm_fp8(x.data_ptr(), x.stride(0), 0 if residual is None else residual.data_ptr(), ldr,
-                              weight.data_ptr(), 0 if residual is None else h.data_ptr(), ldh, at,
-                              0 if y is None else y.data_ptr(), cols, rstd.data_ptr(), rows, cols, eps, code,
-                              _TYPES[weight.dtype], dev.stream)
-    return Normed(h, out.values, out.scales, y, rstd)
+    return Normed(*(_native or _layer()).rms_norm(x, weight, residual, eps, bool(quantized), bool(normed)))
 
 
 def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, *,
@@ -201,56 +93,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
     (the residual stream's gradient), added to dx, which is also the residual's gradient. ``dy`` and
     ``dh`` are of h's shape and type; ``rstd`` and ``h`` are what the forward pass returned. dweight is
     float32."""
-    code = _typed(h, "h")
-    rows, cols = h.shape
-    _like(dy, "dy", h, "h")
-    if dh is not None:
-        _like(dh, "dh", h, "h")
-    _vector(weight, "weight", cols, (h.dtype, torch.float32))
-    _vector(rstd, "rstd", rows, (torch.float32,))
-    with _Device(h, dy, weight, rstd, dh) as dev:
-        dx = torch.empty((rows, cols), dtype=h.dtype, device=h.device)
-        if rows == 0 or cols == 0:
-            return dx, torch.zeros(cols, dtype=torch.float32, device=h.device)
-        dw = torch.empty(cols, dtype=torch.float32, device=h.device)
-        nat = native()
-        work = torch.empty(nat.rms_norm_backward_workspace(rows, cols), dtype=torch.uint8, device=h.device)
-        nat.rms_norm_backward(dy.data_ptr(), dy.stride(0), h.data_ptr(), h.stride(0), weight.data_ptr(), rstd.data_ptr(),
-                              0 if dh is None else dh.data_ptr(), 0 if dh is None else dh.stride(0), dx.data_ptr(),
-                              cols, dw.data_ptr(), work.data_ptr(), rows, cols, code, _TYPES[weight.dtype], dev.stream)
-    return dx, dw
-
-
-def _operand(q, name: str, tiles: bool) -> tuple[torch.Tensor, torch.Tensor, bool, int, int]:
-    """(values, scales, a scale for each 128 x 128, row pitch, scale pitch) of a checked operand."""
-    try:
-        values, scales = q
-    except (TypeError, ValueError):
-        raise TypeError(f"{name} must be a (values, scales) pair, as quantize() returns it") from None
-    _matrix(values, f"{name}'s values")
-    if values.dtype != torch.float8_e4m3fn:
-        raise ValueError(f"{name}'s values must be float8_e4m3fn, not {values.dtype}")
-    if not isinstance(scales, torch.Tensor):
-        raise TypeError(f"{name}'s scales must be a tensor, not {type(scales).__name__}")
-    if scales.dtype != torch.float8_e8m0fnu:
-        raise ValueError(f"{name}'s scales must be float8_e8m0fnu, not {scales.dtype}")
-    rows, cols = values.shape
-    blocks = _up(cols, BLOCK) // BLOCK
-    by_tile = tiles and scales.shape == (_up(rows, BLOCK) // BLOCK, blocks) and scales.shape[0] != rows
-    if not by_tile and scales.shape != (rows, blocks):
-        raise ValueError(f"{name}'s scales must be {(rows, blocks)}{' or a scale for each 128 x 128' if tiles else ''}, "
-                         f"not {tuple(scales.shape)}")
-    ld = values.stride(0) if rows > 1 and cols else _up(cols, 16)
-    if ld % 16 or values.data_ptr() % 16:
-        raise ValueError(f"the rows of {name}'s values must start on 16-byte boundaries, as quantize() lays them out")
-    lds = scales.stride(1) if blocks > 1 else _up(scales.shape[0], 16)
-    room = scales.untyped_storage().nbytes() - scales.storage_offset()
-    if scales.numel() and ((scales.shape[0] > 1 and scales.stride(0) != 1) or lds % 4 or scales.data_ptr() % 4
-                           or (blocks - 1) * lds + _up(scales.shape[0], 4) > room):
-        lds = _up(scales.shape[0], 16)  # the kernels read the scales of one block four rows at a time
-        laid = torch.empty((blocks, lds), dtype=scales.dtype, device=scales.device).t()[:scales.shape[0]]
-        scales = laid.copy_(scales)
-    return values, scales, by_tile, ld, lds
+    return (_native or _layer()).rms_norm_backward(dy, h, weight, rstd, dh)
 
 
 def matmul(a, b, *, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -262,23 +105,4 @@ def matmul(a, b, *, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | Non
     A float32 result is exact to 32-bit sums. For the 16-bit types the matrix instruction lines up 8
     products at a time and drops what is below 2^-13 of the largest, which is far below their rounding
     unless a sum cancels to a thousandth of its terms."""
-    av, asc, _, lda, ldsa = _operand(a, "a", False)
-    bv, bsc, tiles, ldb, ldsb = _operand(b, "b", True)
-    m, k = av.shape
-    n = bv.shape[0]
-    if bv.shape[1] != k:
-        raise ValueError(f"a and b must have as many columns, not {k} and {bv.shape[1]}")
-    if out is not None:
-        _writable(_matrix(out, "out"), "out")
-        if out.shape != (m, n):
-            raise ValueError(f"out must be {(m, n)}, not {tuple(out.shape)}")
-        dtype = out.dtype
-    code = _TYPES.get(dtype)
-    if code is None:
-        raise ValueError(f"the result's dtype must be float32, bfloat16 or float16, not {dtype}")
-    with _Device(av, asc, bv, bsc, out) as dev:
-        c = torch.empty((m, n), dtype=dtype, device=av.device) if out is None else out
-        ldc = c.stride(0) if m > 1 else n
-        native().fp8_matmul((av.data_ptr(), lda, asc.data_ptr(), ldsa), (bv.data_ptr(), ldb, bsc.data_ptr(), ldsb), tiles,
-                            c.data_ptr(), ldc, m, n, k, code, dev.stream)
-    return c
+    return (_native or _layer()).matmul(a, b, dtype, out)

@@ -2,12 +2,14 @@
 
 Outputs (all in-tree so they travel to the GPU box with the repo snapshot):
 
-* ``tritonk8ssupervisor_amd/lib/libtk8s.so`` — HIP kernels (N4-N7) and probes (N1); links only
+* ``tritonk8ssupervisor_amd/lib/libtk8s.so`` — HIP kernels (N4-N7, 8-bit layer) and probes (N1); links only
   ``libamdhip64``.
 * ``tritonk8ssupervisor_amd/lib/libtk8s_rccl.so`` — the RCCL validator (N3); the only artefact
   that links ``librccl`` (573 MB on ROCm 7.2), so the probe and gpuinfo payloads on the
   bring-up's critical path never map it.
 * ``tritonk8ssupervisor_amd/_tk8s_native*.so`` — pybind11 module over both libraries.
+* ``tritonk8ssupervisor_amd/_tk8s_layer*.so`` — the 8-bit layer on torch tensors (ops/fp8.py); built
+  where PyTorch is installed, the only artefact that links it.
 * ``tritonk8ssupervisor_amd/_tk8s_topo*.so`` — pybind11 module of the CPU-only xGMI-aware
   allocator (N2 core); no HIP dependency so the node agent can load it safely.
 * ``tritonk8ssupervisor_amd/bin/tk8s-{gpuinfo,probe,rccl}`` — the validation pod payloads.
@@ -68,6 +70,19 @@ def ext_suffix() -> str:
 
 def native_module_path() -> Path:
     return PKG / f"_tk8s_native{ext_suffix()}"
+
+
+def layer_module_path() -> Path:
+    return PKG / f"_tk8s_layer{ext_suffix()}"
+
+
+def torch_dir() -> Path | None:
+    """Where PyTorch is installed (not imported: that takes seconds), or None."""
+    import importlib.util
+
+    spec = importlib.util.find_spec("torch")
+    where = list(spec.submodule_search_locations or []) if spec else []
+    return Path(where[0]) if where and (Path(where[0]) / "include" / "ATen").is_dir() else None
 
 
 def topo_module_path() -> Path:
@@ -156,6 +171,13 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
     if force or _stale(nat_obj, [nat_src]):
         objs.append((nat_obj, [HIPCC, *COMMON, f"--offload-arch={ARCH}", *py_inc, "-fvisibility=hidden", "-c",
                                str(nat_src), "-o", str(nat_obj)]))
+    torch = torch_dir()  # without PyTorch the 8-bit layer's tensor module is not built
+    layer_obj, layer_src = OBJ / "layer_module.o", NATIVE / "bindings" / "layer_module.cpp"
+    if torch is not None and (force or _stale(layer_obj, [layer_src])):
+        objs.append((layer_obj, [HIPCC, *COMMON, f"--offload-arch={ARCH}", f"-I{sysconfig.get_paths()['include']}",
+                                 "-isystem", str(torch / "include"), "-isystem",
+                                 str(torch / "include" / "torch" / "csrc" / "api" / "include"), "-DUSE_ROCM",
+                                 "-D__HIP_PLATFORM_AMD__", "-fvisibility=hidden", "-c", str(layer_src), "-o", str(layer_obj)]))
     topo_srcs = [NATIVE / "src" / "topology.cpp", NATIVE / "bindings" / "topo_module.cpp"]
     topo_objs = [OBJ / (s.stem + "_topo.o") for s in topo_srcs]
     for s, o in zip(topo_srcs, topo_objs):
@@ -182,6 +204,11 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
     if force or _stale(nat, [nat_obj, lib, rlib]):
         links.append([HIPCC, "-shared", "-fPIC", str(nat_obj), "-o", str(nat), f"-L{LIBDIR}",
                       "-ltk8s_rccl", "-ltk8s", "-Wl,-rpath,$ORIGIN/lib", *hip_libs, "-lrccl"])
+    layer = layer_module_path()
+    if torch is not None and (force or _stale(layer, [layer_obj, lib])):
+        links.append([HIPCC, "-shared", "-fPIC", str(layer_obj), "-o", str(layer), f"-L{LIBDIR}", "-ltk8s",
+                      "-Wl,-rpath,$ORIGIN/lib", f"-L{torch / 'lib'}", f"-Wl,-rpath,{torch / 'lib'}", "-ltorch_python",
+                      "-ltorch_hip", "-ltorch_cpu", "-lc10_hip", "-lc10", *hip_libs])
     topo = topo_module_path()
     if force or _stale(topo, topo_objs):
         links.append([CXX, "-shared", "-fPIC", *[str(o) for o in topo_objs], "-o", str(topo)])
@@ -246,7 +273,8 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
     from .rccl_unpack import unpack
 
     rccl_unpacked = unpack()  # an operator's own RCCL build for the fabric check, if one is kept
-    out = {"libtk8s": lib, "libtk8s_rccl": rlib, "native_module": nat, "topo_module": topo, "tk8s-supervise": sup,
+    out = {"libtk8s": lib, "libtk8s_rccl": rlib, "native_module": nat, "topo_module": topo,
+           **({"layer_module": layer} if torch is not None else {}), "tk8s-supervise": sup,
            "tk8s-gpujail": jail, "tk8s-container": tool_path("tk8s-container"),
            "tk8s-smi": smi, "tk8s-reuse": reuse_bin, "tk8s-hsaprobe": hsa_bin, **cos,
            "rccl-unpacked": rccl_unpacked.get("path") or f"no ({rccl_unpacked.get('why')})"}
