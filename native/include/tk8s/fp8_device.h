@@ -18,6 +18,98 @@ constexpr int kScaleBlock = 128;  // values that share a scale, along a row (or 
 // (global memory takes them at every address), so an odd row pitch costs no separate kernel.
 template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Eight { T v[8]; };
 
+// The same 8 values as they are stored, in whole registers: 16-bit values two to a dword.
+template <class T> struct Packed8 { unsigned d[2 * sizeof(T)]; };
+
+template <class T> __device__ __forceinline__ float unpack(const Packed8<T>& p, int j) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(p.d[j]);
+  } else if constexpr (__is_same(T, __bf16)) {
+    return __uint_as_float(j % 2 ? p.d[j / 2] & 0xffff0000u : p.d[j / 2] << 16);
+  } else {
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(p.d[j / 2] >> (16 * (j % 2)))));
+  }
+}
+
+// Two values, rounded to T, into dword i (of 16-bit values), or one into each of two.
+template <class T> __device__ __forceinline__ void pack(Packed8<T>& p, int i, float v0, float v1) {
+  if constexpr (sizeof(T) == 4) {
+    p.d[2 * i] = __float_as_uint(v0);
+    p.d[2 * i + 1] = __float_as_uint(v1);
+  } else {
+    typedef T Two __attribute__((ext_vector_type(2)));
+    const Two t = {static_cast<T>(v0), static_cast<T>(v1)};
+    p.d[i] = __builtin_bit_cast(unsigned, t);
+  }
+}
+
+template <int kAlign> struct Dwords;
+template <> struct Dwords<2> { typedef unsigned four __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Dwords<4> { typedef unsigned four __attribute__((ext_vector_type(4), aligned(4))); };
+
+// Whole dwords from (to) an address of any element, past the caches: what is streamed is touched once.
+template <class T> __device__ __forceinline__ Packed8<T> at_any(const T* p) {
+  typedef typename Dwords<sizeof(T)>::four Four;
+  Packed8<T> e;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+    const Four u = __builtin_nontemporal_load(reinterpret_cast<const Four*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e.d[4 * i + j] = u[j];
+  }
+  return e;
+}
+
+template <class T> __device__ __forceinline__ void at_any(T* p, const Packed8<T>& e) {
+  typedef typename Dwords<sizeof(T)>::four Four;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+    const Four u = {e.d[4 * i], e.d[4 * i + 1], e.d[4 * i + 2], e.d[4 * i + 3]};
+    __builtin_nontemporal_store(u, reinterpret_cast<Four*>(p) + i);
+  }
+}
+
+// p[0..n-1], zeros behind; n <= 0 reads nothing. kWhole: n is 8 or more, or 0 or less.
+template <bool kWhole, class T> __device__ __forceinline__ Packed8<T> load_packed(const T* p, int n) {
+  Packed8<T> e = {};
+  if (kWhole ? n > 0 : n >= 8) {
+    e = at_any(p);
+  } else if (!kWhole && n > 0) {
+    Eight<T> o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o.v[j] = j < n ? p[j] : static_cast<T>(0.f);
+    e = __builtin_bit_cast(Packed8<T>, o);
+  }
+  return e;
+}
+
+template <bool kWhole, class T> __device__ __forceinline__ void store_packed(T* p, int n, const Packed8<T>& e) {
+  if (kWhole ? n > 0 : n >= 8) {
+    at_any(p, e);
+  } else if (!kWhole) {
+    const Eight<T> o = __builtin_bit_cast(Eight<T>, e);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = o.v[j];
+  }
+}
+
+// Keeps the compiler from unpacking a loop's constants into twice the registers before it.
+template <class T> __device__ __forceinline__ void keep_packed(Packed8<T>& p) {
+  if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(p.d[0]), "+v"(p.d[1]), "+v"(p.d[2]), "+v"(p.d[3]));
+}
+
+// 8 bytes of e4m3 to where n of them belong.
+template <bool kWhole> __device__ __forceinline__ void store_bytes(uint8_t* p, int n, u32x2 v) {
+  if (kWhole ? n > 0 : n >= 8) {
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x2*>(p));
+  } else if (!kWhole) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = static_cast<uint8_t>((j < 4 ? v.x : v.y) >> (8 * (j & 3)));
+  }
+}
+
 // v[0..7] = p[0..n-1], zeros behind; n <= 0 reads nothing.
 template <class T> __device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
   if (n >= 8) {
@@ -54,6 +146,15 @@ __device__ __forceinline__ float round_to_odd(double v) {
   return static_cast<float>(__longlong_as_double(static_cast<unsigned long long>(hi) << 32));
 }
 
+// 1 / sqrt(x) to the last bits of 64: the instruction's first 2^-25 or so, then one step of third order.
+// 0 and infinity keep what the instruction says.
+__device__ __forceinline__ double inverse_sqrt(double x) {
+  const double r = __builtin_amdgcn_rsq(x);
+  const double e = fma(-x * r, r, 1.0);
+  const double better = fma(r * e, fma(0.375, e, 0.5), r);
+  return x > 0.0 && x < __builtin_inf() ? better : r;
+}
+
 __device__ __forceinline__ unsigned magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // E8M0 byte of a block whose largest magnitude has these float bits (the bits order as the values
@@ -78,13 +179,115 @@ __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d, un
   return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, r, true));
 }
 
+// Whether a 32-bit value that may be kSlack units in its last place off could round to another e4m3
+// value than the exact one, or its block get another scale: the borders between e4m3 values are
+// numbers whose low 19 fraction bits are 0 (those between scales, 448 2^e, too).
+constexpr unsigned kSlack = 4;
+__device__ __forceinline__ unsigned from_border(float v) { return (__float_as_uint(v) + kSlack) & 0x7ffffu; }
+__device__ __forceinline__ bool near_border(unsigned least) { return least <= 2 * kSlack; }
+
+// Magnitudes of 8 stored values, compared as they are stored: 16-bit ones two to a dword (their bits,
+// sign off, order as the values do, NaN above infinity).
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+template <class T> __device__ __forceinline__ Packed8<T> magnitudes(const Packed8<T>& v) {
+  Packed8<T> m;
+#pragma unroll
+  for (int i = 0; i < 2 * static_cast<int>(sizeof(T)); ++i) m.d[i] = v.d[i] & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu);
+  return m;
+}
+
+template <class T> __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {  // of one dword
+  if constexpr (sizeof(T) == 2)
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+  else
+    return max(a, b);
+}
+
+template <class T> __device__ __forceinline__ Packed8<T> larger(const Packed8<T>& a, const Packed8<T>& b) {
+  Packed8<T> m;
+#pragma unroll
+  for (int i = 0; i < 2 * static_cast<int>(sizeof(T)); ++i) m.d[i] = larger<T>(a.d[i], b.d[i]);
+  return m;
+}
+
+// The bits, as a float's, of magnitude j; of the largest of the 8.
+template <class T> __device__ __forceinline__ unsigned magnitude_of(const Packed8<T>& m, int j) { return __float_as_uint(unpack(m, j)); }
+
+template <class T> __device__ __forceinline__ unsigned largest_of(const Packed8<T>& m) {
+  unsigned v = m.d[0];
+#pragma unroll
+  for (int i = 1; i < 2 * static_cast<int>(sizeof(T)); ++i) v = larger<T>(v, m.d[i]);
+  if constexpr (sizeof(T) == 2) {
+    const unsigned top = max(v & 0xffffu, v >> 16);
+    if constexpr (__is_same(T, __bf16)) return top << 16;
+    else return __float_as_uint(static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(top))));
+  } else {
+    return v;
+  }
+}
+
+// Four e4m3 bytes of values 4 i .. 4 i + 3 under one block's scale. 16-bit values go through the conversion
+// that takes the scale's exponent along; its ends (2^-127 and NaN) go the long way.
+template <class T> __device__ __forceinline__ unsigned pack_four(const Packed8<T>& v, int i, unsigned byte) {
+  if constexpr (sizeof(T) == 2) {
+    if (byte - 1u < 254u) {
+      typedef short Old __attribute__((ext_vector_type(2)));
+      typedef T Two __attribute__((ext_vector_type(2)));
+      const float scale = __uint_as_float(byte << 23);
+      Old r = {0, 0};
+      if constexpr (__is_same(T, __bf16)) {
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(Two, v.d[2 * i]), scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(Two, v.d[2 * i + 1]), scale, true);
+      } else {
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(Two, v.d[2 * i]), scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(Two, v.d[2 * i + 1]), scale, true);
+      }
+      return __builtin_bit_cast(unsigned, r);
+    }
+  }
+  return pack4(unpack(v, 4 * i), unpack(v, 4 * i + 1), unpack(v, 4 * i + 2), unpack(v, 4 * i + 3), byte);
+}
+
+// Column j of 8 rows of 8 values, as 8 stored values.
+template <class T> __device__ __forceinline__ Packed8<T> column(const Packed8<T> (&v)[8], int j) {
+  Packed8<T> c;
+#pragma unroll
+  for (int i = 0; i < 2 * static_cast<int>(sizeof(T)); ++i) {
+    if constexpr (sizeof(T) == 2) c.d[i] = __builtin_amdgcn_perm(v[2 * i + 1].d[j / 2], v[2 * i].d[j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+    else c.d[i] = v[i].d[j];
+  }
+  return c;
+}
+
+// v of the lane kBy places on within its 16, on the vector unit's own crossbar.
+template <int kBy> __device__ __forceinline__ unsigned rotate16(unsigned v) {
+  return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x120 + kBy, 0xf, 0xf, false));
+}
+
 // The largest over the 16 lanes that hold one block.
 __device__ __forceinline__ unsigned max16(unsigned v) {
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) {
-    const unsigned o = __shfl_xor(v, off, 64);
-    v = o > v ? o : v;
-  }
+  v = max(v, rotate16<8>(v));
+  v = max(v, rotate16<4>(v));
+  v = max(v, rotate16<2>(v));
+  return max(v, rotate16<1>(v));
+}
+
+template <int kBy> __device__ __forceinline__ float rotate16(float v) { return __uint_as_float(rotate16<kBy>(__float_as_uint(v))); }
+template <int kBy> __device__ __forceinline__ double rotate16(double v) {
+  const unsigned long long b = __double_as_longlong(v);
+  const unsigned long long lo = rotate16<kBy>(static_cast<unsigned>(b)), hi = rotate16<kBy>(static_cast<unsigned>(b >> 32));
+  return __longlong_as_double(hi << 32 | lo);
+}
+
+// The sum over kLanes (16, 32 or 64) neighbouring lanes, the same in all of them and in every call.
+template <int kLanes, class V> __device__ __forceinline__ V sum_lanes(V v) {
+  v += rotate16<8>(v);
+  v += rotate16<4>(v);
+  v += rotate16<2>(v);
+  v += rotate16<1>(v);
+  if constexpr (kLanes >= 32) v += __shfl_xor(v, 16, 64);
+  if constexpr (kLanes >= 64) v += __shfl_xor(v, 32, 64);
   return v;
 }
 
