@@ -70,119 +70,166 @@ __device__ __forceinline__ float scale_value(unsigned byte) { return __uint_as_f
 // (or beyond what a 32-bit C could hold). Others, and NaN, take the way through ldexp.
 __device__ __forceinline__ bool far_scale(unsigned byte) { return byte - 27u > 200u; }
 
+// Of the four scales of a dword those of rows below count, the first being row `first`; 2^0 for the others,
+// whose bytes are anything: they must not decide which way the sums go.
+__device__ __forceinline__ unsigned own_scales(unsigned scales, size_t first, size_t count) {
+  const size_t n = first < count ? count - first : 0;
+  const unsigned keep = n >= 4 ? ~0u : (1u << (8 * n)) - 1;
+  return (scales & keep) | (0x7f7f7f7fu & ~keep);
+}
+
 // part * 2^(sa + sb - 254), NaN for a NaN scale.
 __device__ __forceinline__ float scaled(float part, unsigned sa, unsigned sb) {
   if (sa == 255u || sb == 255u) return __uint_as_float(0x7fc00000u);
   return ldexpf(part, static_cast<int>(sa + sb) - 254);
 }
 
-// 16 bytes of a row at k, zeros from k_end on; reads no byte behind k_end.
+// 16 bytes of a row at k, zeros from k_end on. Rows start on 16 bytes and so does k: the 16 bytes that hold
+// the row's last value lie in one page with it, and what is read behind it is masked off.
 __device__ __forceinline__ u32x4 load16(const uint8_t* row, size_t k, size_t k_end) {
-  if (k + 16 <= k_end) return *reinterpret_cast<const u32x4*>(row + k);
-  u32x4 r = {0, 0, 0, 0};
-  for (int j = 0; k + j < k_end; ++j) r[j / 4] |= static_cast<unsigned>(row[k + j]) << (8 * (j % 4));
+  u32x4 r = *reinterpret_cast<const u32x4*>(row + std::min(k, (k_end - 1) / 16 * 16));
+  const int n = k < k_end ? static_cast<int>(std::min<size_t>(k_end - k, 16)) : 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] &= n >= 4 * j + 4 ? ~0u : n <= 4 * j ? 0u : (1u << (8 * (n - 4 * j))) - 1;
   return r;
 }
 
 // ------------------------------------------------------------------------------------------
 // Few rows of A
 // ------------------------------------------------------------------------------------------
-// The weights are read once and nothing else matters. A block makes 16 columns of C; its waves share
-// them along k, wave w the blocks w, w + WAVES, ..., so the block reads whole rows in order, and join
-// their sums in LDS in the order of the waves. B and A go from memory to registers directly (A
-// is small and stays in L2), kAhead steps requested at a time.
-template <class O, bool kExact, int MT, int WAVES, int kAhead>
+// The weights are read once and that is what it should take. A block makes 16 NT columns of C; its waves
+// share them along k, wave w the blocks w, w + WAVES, ..., so the block reads whole rows in order, and
+// join their sums in LDS in the order of the waves. B and A go from memory to registers directly;
+// kAhead of a wave's blocks are on their way at any time. A is small and stays in L2, but every block
+// reads all of it, and from rows a power of two apart that is slow (27 x 8192 by 8192 columns: 17 us for
+// A alone, 14 for B alone): NT = 2 halves it.
+template <class O, bool kExact, int MT, int NT, int WAVES, int kAhead>
 __global__ __launch_bounds__(WAVES * 64) void matmul_rows_kernel(MatmulArgs a) {
-  __shared__ float part[WAVES][MT * 256];
+  __shared__ float part[WAVES][NT * MT * 256];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, group = lane / 16;
-  const size_t n0 = static_cast<size_t>(blockIdx.x) * 16, m0 = static_cast<size_t>(blockIdx.y) * (16 * MT);
+  const size_t n0 = static_cast<size_t>(blockIdx.x) * (16 * NT), m0 = static_cast<size_t>(blockIdx.y) * (16 * MT);
   const size_t nb = (a.k + kScaleBlock - 1) / kScaleBlock;
   const size_t whole = a.k / kScaleBlock;  // blocks with all their values
-  const size_t n = std::min(n0 + lane % 16, a.n - 1);  // what is behind the last row is computed, not stored
-  const uint8_t* const brow = a.b.values + n * a.b.ld + 16 * group;
-  const uint8_t* const bscale = a.b.scales + (a.b_tiles ? n / kScaleBlock : n);
-  const uint8_t* arow[MT];
-  const uint8_t* ascale[MT];
+  const uint8_t *brow[NT], *bscale[NT], *arow[MT], *ascale[MT];  // what is behind the last row is computed, not stored
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const size_t n = std::min(n0 + 16 * j + lane % 16, a.n - 1);
+    brow[j] = a.b.values + n * a.b.ld + 16 * group;
+    bscale[j] = a.b.scales + (a.b_tiles ? n / kScaleBlock : n);
+  }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const size_t m = std::min(m0 + 16 * i + lane % 16, a.m - 1);
     arow[i] = a.a.values + m * a.a.ld + 16 * group;
     ascale[i] = a.a.scales + m;
   }
-  f32x4 acc[MT];
+  f32x4 acc[NT][MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto step = [&](const Fragment& fb, const Fragment (&fa)[MT], unsigned sb, const unsigned (&sa)[MT]) {
+  auto step = [&](const Fragment (&fb)[NT], const Fragment (&fa)[MT], const unsigned (&sb)[NT], const unsigned (&sa)[MT]) {
     if constexpr (!kExact) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb.v, fa[i].v, acc[i], 0, 0, 0, static_cast<int>(sb), 0,
-                                                                 static_cast<int>(sa[i]));
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa[i].v, acc[j][i], 0, 0, 0, static_cast<int>(sb[j]), 0,
+                                                                      static_cast<int>(sa[i]));
     } else {
-      bool far = far_scale(sb);
+      bool far = false;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) far |= far_scale(sa[i]);
-      if (__builtin_amdgcn_ballot_w64(far) == 0) {
-        const Wide wb = widen(fb, scale_value(sb));
+      for (int j = 0; j < NT; ++j) far = far || far_scale(sb[j]);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i] = multiply(wb, widen(fa[i], scale_value(sa[i])), acc[i]);
-      } else {
-        const Wide wb = widen(fb, 1.f);
+      for (int i = 0; i < MT; ++i) far = far || far_scale(sa[i]);
+      const bool near = __builtin_amdgcn_ballot_w64(far) == 0;
+      Wide wb[NT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const f32x4 p = multiply(wb, widen(fa[i], 1.f), f32x4{0.f, 0.f, 0.f, 0.f});
+      for (int j = 0; j < NT; ++j) wb[j] = widen(fb[j], near ? scale_value(sb[j]) : 1.f);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][r] += scaled(p[r], sa[i], __shfl(sb, 4 * group + r, 64));
+      for (int i = 0; i < MT; ++i) {
+        const Wide wa = widen(fa[i], near ? scale_value(sa[i]) : 1.f);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          if (near) {
+            acc[j][i] = multiply(wb[j], wa, acc[j][i]);
+          } else {
+            const f32x4 p = multiply(wb[j], wa, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[j][i][r] += scaled(p[r], sa[i], __shfl(sb[j], 4 * group + r, 64));
+          }
         }
       }
     }
   };
 
-  size_t b = wave;
-  for (; b + (kAhead - 1) * WAVES < whole; b += kAhead * WAVES) {
-    Fragment fb[kAhead], fa[kAhead][MT];
-    unsigned sb[kAhead], sa[kAhead][MT];
+  // This wave's whole blocks: wave, wave + WAVES, ..., from a place of the block's own on and round, so that
+  // the blocks do not all ask the same channel of L2 for the same piece of A (27 x 8192: 22 -> 20 us).
+  // Loads come back in the order of their requests, so A's are made as early as B's, though A is near.
+  const unsigned steps = whole > static_cast<size_t>(wave) ? static_cast<unsigned>((whole - wave + WAVES - 1) / WAVES) : 0;
+  Fragment fb[kAhead][NT], fa[kAhead][MT];
+  unsigned sb[kAhead][NT], sa[kAhead][MT];
+  const unsigned turn = steps ? blockIdx.x & ((1u << (31 - __builtin_clz(steps))) - 1) : 0;
+  auto request = [&](unsigned s, int u) {
+    unsigned q = (s < steps ? s : steps - 1) + turn;
+    q = q >= steps ? q - steps : q;
+    const size_t at = wave + static_cast<size_t>(q) * WAVES;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const size_t at = b + u * WAVES;
-      fb[u].half[0] = *reinterpret_cast<const u32x4*>(brow + at * kScaleBlock);
-      fb[u].half[1] = *reinterpret_cast<const u32x4*>(brow + at * kScaleBlock + 64);
-      sb[u] = bscale[at * a.b.ld_scales];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        fa[u][i].half[0] = *reinterpret_cast<const u32x4*>(arow[i] + at * kScaleBlock);
-        fa[u][i].half[1] = *reinterpret_cast<const u32x4*>(arow[i] + at * kScaleBlock + 64);
-        sa[u][i] = ascale[i][at * a.a.ld_scales];
-      }
+    for (int j = 0; j < NT; ++j) {
+      fb[u][j].half[0] = *reinterpret_cast<const u32x4*>(brow[j] + at * kScaleBlock);
+      fb[u][j].half[1] = *reinterpret_cast<const u32x4*>(brow[j] + at * kScaleBlock + 64);
+      sb[u][j] = bscale[j][at * a.b.ld_scales];
     }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) step(fb[u], fa[u], sb[u], sa[u]);
-  }
-  for (; b < nb; b += WAVES) {  // what is left, the block cut off by the end of the rows included
-    Fragment fb, fa[MT];
-    unsigned sa[MT];
-    const size_t k = b * kScaleBlock + 16 * group;
-    fb.half[0] = load16(brow - 16 * group, k, a.k);
-    fb.half[1] = load16(brow - 16 * group, k + 64, a.k);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      fa[i].half[0] = load16(arow[i] - 16 * group, k, a.k);
-      fa[i].half[1] = load16(arow[i] - 16 * group, k + 64, a.k);
-      sa[i] = ascale[i][b * a.a.ld_scales];
+      fa[u][i].half[0] = *reinterpret_cast<const u32x4*>(arow[i] + at * kScaleBlock);
+      fa[u][i].half[1] = *reinterpret_cast<const u32x4*>(arow[i] + at * kScaleBlock + 64);
+      sa[u][i] = ascale[i][at * a.a.ld_scales];
     }
-    step(fb, fa, bscale[b * a.b.ld_scales], sa);
+  };
+  if (steps) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) request(u, u);
+    for (unsigned s = 0; s < steps; s += kAhead) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (u && s + u >= steps) break;
+        step(fb[u], fa[u], sb[u], sa[u]);
+        if (s + u + kAhead < steps) request(s + u + kAhead, u);
+      }
+    }
+  }
+  const size_t b = wave + static_cast<size_t>(steps) * WAVES;
+  if (b < nb) {  // the block cut off by the end of the rows, if it is this wave's
+    const size_t k = b * kScaleBlock + 16 * group;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      fb[0][j].half[0] = load16(brow[j] - 16 * group, k, a.k);
+      fb[0][j].half[1] = load16(brow[j] - 16 * group, k + 64, a.k);
+      sb[0][j] = bscale[j][b * a.b.ld_scales];
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      fa[0][i].half[0] = load16(arow[i] - 16 * group, k, a.k);
+      fa[0][i].half[1] = load16(arow[i] - 16 * group, k + 64, a.k);
+      sa[0][i] = ascale[i][b * a.a.ld_scales];
+    }
+    step(fb[0], fa[0], sb[0], sa[0]);
   }
 
   // lane: row lane % 16 of A, columns 4 * group .. + 3
 #pragma unroll
-  for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(&part[wave][i * 256 + (lane % 16) * 16 + 4 * group]) = acc[i];
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      *reinterpret_cast<f32x4*>(&part[wave][(j * MT + i) * 256 + (lane % 16) * 16 + 4 * group]) = acc[j][i];
   __syncthreads();
-  for (int e = threadIdx.x; e < MT * 256; e += WAVES * 64) {
+  for (int e = threadIdx.x; e < NT * MT * 256; e += WAVES * 64) {
     float s = part[0][e];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) s += part[w][e];
-    const size_t row = m0 + e / 16, col = n0 + e % 16;
+    const size_t row = m0 + e / 256 % MT * 16 + e % 256 / 16, col = n0 + e / 256 / MT * 16 + e % 16;
     if (row < a.m && col < a.n) static_cast<O*>(a.c)[row * a.ldc + col] = static_cast<O>(s);
   }
 }
@@ -413,6 +460,7 @@ __global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(
 
   // A step loaded with zeros behind the end of the rows, everything waited for.
   auto load_slowly = [&](unsigned b) {
+#pragma unroll 2
     for (int q = wave; q < kRows; q += kWaves) {
       const int r = slot_row(8 * q + lane / 8);
       const size_t k = static_cast<size_t>(b) * kScaleBlock + 16 * ((lane % 8) ^ (r / 4 % 8));
@@ -477,10 +525,11 @@ __global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(
     // Two groups of waves take turns, one phase apart: while one reads a step and widens B, the other
     // multiplies. A slot is refilled when the later group has read it. All waves look at all scales
     // of a step, so they give up together when one is far and make the tile again the slow way.
-    static_assert(kStages == 3 && kWaves == 8, "two groups");
+    static_assert(kStages == 3 && kWaves == 8 && TN == kScaleBlock, "two groups, one tile of B's scales");
     auto all_near = [&](unsigned slot) {
       const unsigned* const scales = reinterpret_cast<const unsigned*>(lds + slot * kSlot + kScales);
-      const unsigned va = scales[lane % (TM / 4)], vb = scales[64 + (a.b_tiles ? lane % 2 : lane % (TN / 4))];
+      const unsigned va = own_scales(scales[lane % (TM / 4)], m0 + 4 * (lane % (TM / 4)), a.m);
+      const unsigned vb = a.b_tiles ? __builtin_amdgcn_perm(0, scales[64], pick) : own_scales(scales[64 + lane % (TN / 4)], n0 + 4 * (lane % (TN / 4)), a.n);
       bool far = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) far = far || far_scale(va >> (8 * i) & 255u) || far_scale(vb >> (8 * i) & 255u);
@@ -548,6 +597,174 @@ __global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(
     }
   }
   store(acc);
+}
+
+// ------------------------------------------------------------------------------------------
+// Small tiles, shared along k
+// ------------------------------------------------------------------------------------------
+// Where larger tiles would leave most of the chip idle: a block makes 64 x 64 of C, and each of its four
+// waves takes every fourth step of 128 k for itself -- its own two slots in LDS, filled two steps
+// ahead and waited for by count, no barrier -- with the four sums joined in LDS at the end, in order.
+constexpr int kSplit = 4;
+constexpr int kSplitSlot = 128 * 128 + 256;  // 64 rows of A, 64 of B, 16 dwords of scales of each (and room)
+constexpr int kSplitPitch = 68;              // floats of a row of partial sums
+
+// A dword for each lane from its own address to LDS.
+__device__ __forceinline__ void load_lds4_each(unsigned to, const uint8_t* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
+}
+
+template <class O, bool kExact>
+__global__ __launch_bounds__(kSplit * 64, 1) void matmul_split_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kSplit * 2 * kSplitSlot];
+  static_assert(kSplit * 64 * kSplitPitch * 4 <= kSplit * 2 * kSplitSlot, "the partial sums go where the steps were");
+  const int lane = threadIdx.x % 64, group = lane / 16, j16 = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  unsigned tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const size_t m0 = static_cast<size_t>(tm) * 64, n0 = static_cast<size_t>(tn) * 64;
+  const unsigned whole = static_cast<unsigned>(a.k / kScaleBlock);
+  const unsigned steps = whole > static_cast<unsigned>(wave) ? (whole - wave + kSplit - 1) / kSplit : 0;
+  uint8_t* const mine = lds + wave * 2 * kSplitSlot;
+  const unsigned lds0 = lds_address(mine);
+
+  const uint8_t* const abase = a.a.values + m0 * a.a.ld;
+  const uint8_t* const bbase = a.b.values + n0 * a.b.ld;
+  unsigned off_a[8], off_b[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const int r = slot_row(8 * c + lane / 8);
+    const unsigned piece = 16u * ((lane % 8) ^ (r / 4 % 8));
+    off_a[c] = static_cast<unsigned>(std::min<size_t>(r, a.m - 1 - m0)) * static_cast<unsigned>(a.a.ld) + piece;
+    off_b[c] = static_cast<unsigned>(std::min<size_t>(r, a.n - 1 - n0)) * static_cast<unsigned>(a.b.ld) + piece;
+  }
+  // scales: lanes 0-15 a dword of A's rows each, 16-31 of B's (for 128 x 128 tiles of B the same one, with
+  // this tile's byte in it); the others repeat them
+  const bool of_b = lane / 16 % 2;
+  const size_t tile_n = n0 / kScaleBlock;
+  const uint8_t* const scales = !of_b       ? a.a.scales + std::min(m0 + 4 * j16, (a.m - 1) / 4 * 4)
+                                : a.b_tiles ? a.b.scales + tile_n / 4 * 4
+                                            : a.b.scales + std::min(n0 + 4 * j16, (a.n - 1) / 4 * 4);
+  const size_t scale_step = of_b ? a.b.ld_scales : a.a.ld_scales;
+  const unsigned pick = a.b_tiles ? static_cast<unsigned>(tile_n % 4) * 0x01010101u : 0x03020100u;
+
+  constexpr int kLoads = 17;
+  auto load = [&](unsigned s, unsigned slot, int c) {  // behind the last step it is read once more, for the counts
+    const size_t b = static_cast<size_t>(s < steps ? s : steps - 1) * kSplit + wave;
+    const unsigned to = lds0 + slot * kSplitSlot;
+    if (c == 0) load_lds4_each(to + 128 * 128, scales + b * scale_step);
+    else if (c < 9) load_lds16(to + (c - 1) * 1024, abase + b * kScaleBlock, off_a[c - 1]);
+    else load_lds16(to + (c - 1) * 1024, bbase + b * kScaleBlock, off_b[c - 9]);
+  };
+  unsigned lane_at[2][2];
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      lane_at[odd][h] = lds0 + 512u * j16 + 128u * (odd ^ (j16 / 8)) + 16u * ((4 * h + group) ^ (j16 % 8));
+  auto read_scales = [&](unsigned slot, Operands& f) {
+    const unsigned* const at = reinterpret_cast<const unsigned*>(mine + slot * kSplitSlot + 128 * 128);
+    f.sa = own_scales(at[j16], m0 + 4 * j16, a.m);
+    f.sb = __builtin_amdgcn_perm(0, at[16 + j16], pick);
+    if (!a.b_tiles) f.sb = own_scales(f.sb, n0 + 4 * j16, a.n);
+  };
+  auto read_piece = [&](unsigned slot, Operands& f, int c) {  // piece c of the 16: B's, then A's
+    typedef const __attribute__((address_space(3))) u32x4* lds16;
+    const int i = c / 2 % 4, h = c % 2;
+    if (c < 8) f.b[i].half[h] = *reinterpret_cast<lds16>(lane_at[i % 2][h] + slot * kSplitSlot + 8192 + i / 2 * 256);
+    else f.a[i].half[h] = *reinterpret_cast<lds16>(lane_at[i % 2][h] + slot * kSplitSlot + i / 2 * 256);
+  };
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Operands f[2];
+  auto multiply_exactly = [&](const Operands& o) {
+    bool far = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) far = far || far_scale(o.sb >> (8 * i) & 255u) || far_scale(o.sa >> (8 * i) & 255u);
+    const bool near = __builtin_amdgcn_ballot_w64(far) == 0;
+    Wide wb[4];
+    widen_b(o, near ? o.sb : 0x7f7f7f7fu, wb);
+    if (near) multiply_wide(o, wb, acc);
+    else scaled_sums(o, wb, acc, group);
+  };
+
+  if (steps) {
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) load(0, 0, c);
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) load(1, 1, c);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+    read_scales(0, f[0]);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) read_piece(0, f[0], c);
+    auto step = [&](unsigned s, const Operands& now, Operands& then) {
+      const unsigned next = (s + 1) % 2;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // step s is in registers: its slot is free
+#pragma unroll
+      for (int c = 0; c < kLoads; ++c) load(s + 2, s % 2, c);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");  // step s + 1 is in LDS
+      read_scales(next, then);
+      if constexpr (kExact) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) read_piece(next, then, c);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply_exactly(now);
+      } else {
+        multiply_step(now, acc, [&](int c) { read_piece(next, then, c); });
+      }
+    };
+    for (unsigned s = 0; s < steps; s += 2) {
+      step(s, f[0], f[1]);
+      if (s + 1 < steps) step(s + 1, f[1], f[0]);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
+  if (a.k % kScaleBlock && whole % kSplit == static_cast<unsigned>(wave)) {  // the block cut off by the end of the rows
+    const size_t k = static_cast<size_t>(whole) * kScaleBlock;
+#pragma unroll 8
+    for (int c = 0; c < 16; ++c) {
+      const int r = slot_row(8 * (c % 8) + lane / 8);
+      const size_t piece = 16 * ((lane % 8) ^ (r / 4 % 8));
+      const uint8_t* const src = c < 8 ? a.a.values + std::min(m0 + r, a.m - 1) * a.a.ld : a.b.values + std::min(n0 + r, a.n - 1) * a.b.ld;
+      *reinterpret_cast<u32x4*>(mine + c * 1024 + lane * 16) = load16(src, k + piece, a.k);
+    }
+    load_lds4_each(lds0 + 128 * 128, scales + whole * scale_step);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    read_scales(0, f[0]);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) read_piece(0, f[0], c);
+    if constexpr (kExact) multiply_exactly(f[0]);
+    else multiply_step(f[0], acc, [](int) {});
+  }
+
+  __syncthreads();  // everyone has read its last step
+  float* const part = reinterpret_cast<float*>(lds) + wave * 64 * kSplitPitch;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<f32x4*>(part + (4 * j16 + i) * kSplitPitch + 16 * group + 4 * r) =
+          f32x4{acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]};
+  __syncthreads();
+  const int row = wave * 16 + lane / 4, col = lane % 4 * 16;  // 16 columns of a row each
+  if (m0 + row >= a.m) return;
+  const float* const sums = reinterpret_cast<const float*>(lds) + row * kSplitPitch + col;
+  O* const c = static_cast<O*>(a.c) + (m0 + row) * a.ldc + n0 + col;
+  const int left = a.n > n0 + col ? static_cast<int>(std::min<size_t>(a.n - n0 - col, 16)) : 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = sums[8 * h + e];
+#pragma unroll
+      for (int w = 1; w < kSplit; ++w) v[e] += sums[w * 64 * kSplitPitch + 8 * h + e];
+    }
+    store8(c + 8 * h, left - 8 * h, v);
+  }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -708,7 +925,7 @@ __global__ __launch_bounds__(512, 2) void matmul_big_kernel(MatmulArgs a, unsign
   };
 
   if (a.k % kScaleBlock) {  // first the block that the end of the rows cuts off, zeros behind it
-#pragma unroll 1
+#pragma unroll
     for (int c = 0; c < 8; ++c) {
       const int row = static_cast<int>(r) + (c < 4 ? 64 * c : (c - 4) % 2 * 128 + (c - 4) / 2 * 64);
       const uint8_t* const src = c < 4 ? a.b.values + std::min(n0 + row, a.n - 1) * a.b.ld : a.a.values + std::min(m0 + row, a.m - 1) * a.a.ld;
@@ -782,27 +999,71 @@ template <class O, bool kExact, int TM, int TN, int kStages> void launch_stage(c
                      0, stream, a, static_cast<unsigned>(tm), static_cast<unsigned>(tn));
 }
 
+template <class O, bool kExact, int MT, int NT, int WAVES, int kAhead> void launch_rows(const MatmulArgs& a, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((a.n + 16 * NT - 1) / (16 * NT)), static_cast<unsigned>((a.m + 16 * MT - 1) / (16 * MT)));
+  hipLaunchKernelGGL((matmul_rows_kernel<O, kExact, MT, NT, WAVES, kAhead>), grid, dim3(WAVES * 64), 0, stream, a);
+}
+
+// Which tile makes a product: each kernel has one block on a CU at a time, so it takes
+// ceil(tiles / 256) rounds, each of a start and an end and a time for every 128 k. The figures in launch() are
+// microseconds measured on whole rounds; 16-bit products of k = 4096 with n = 4096 (and a few others):
+//
+//     m x n x k          64 x 64 (k shared)   128 x 128   256 x 128   256 x 256
+//     100 x 8192 x 2048        7.9                -           -           -      (rows kernel 16.5)
+//     256 x 4096 x 4096       12.1              19.8        29.8        50.7
+//     500 x 500 x 8000        17.7              33.1          -           -      (rows kernel 24.3)
+//     512 x 4096 x 4096       20.4              21.0        31.3        51.3
+//     2000 x 2000 x 2000      31.5              21.3        26.1        36.7
+//     1024 x 4096 x 4096      38.4              24.6        33.4        53.3
+//     777 x 5003 x 4432       57.6              47.6        39.5        58.1
+//     2048 x 4096 x 4096      74.0              50.5        39.4        57.2
+//     8192 x 1024 x 8192     132.5             104.2        74.0        97.4
+//     4096 x 4096 x 4096        -               110          85          69.3
+//
+// and float32 ones, 64 x 64 against 256 x 128: 100 x 4096 x 4096 19.6 and 49.3, 1000 x 1000 x 8000 36.4 and
+// 96.9, 1024 x 4096 x 4096 78.3 and 61.2, 2048 x 4096 x 4096 152.5 and 79.9.
+struct Tiles {
+  unsigned m, n;
+  Tiles(const MatmulArgs& a, size_t tm, size_t tn) : m(static_cast<unsigned>((a.m + tm - 1) / tm)), n(static_cast<unsigned>((a.n + tn - 1) / tn)) {}
+  dim3 grid() const { return dim3(m * n); }
+  double time(double ends, double step, size_t steps) const {
+    const size_t rounds = (static_cast<size_t>(m) * n + 255) / 256;
+    return static_cast<double>(rounds) * (ends + step * static_cast<double>(steps));
+  }
+};
+
 template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t stream) {
-  const bool tiled = a.m > 32 && a.a.ld < (1u << 23) && a.b.ld < (1u << 23);
+  // Rows too long for the tiles' 32-bit offsets, and few rows of A: the tiles of 64 columns leave most CUs
+  // without one while n <= 6144 (16-bit, 24 x 4096 x 4096: rows 7.9 us, tiles 9.0; 64 x 4096 x 4096 13.9 and
+  // 9.1; 24 x 14336 x 4096 18.2 and 13.4), and they are slow at float32 (64 x 4096 x 4096: 13.1 and 18.9).
+  const bool tiled = a.a.ld < (1u << 23) && a.b.ld < (1u << 23) && (a.m > 64 || (!kExact && (a.m > 32 || a.n > 6144)));
   if (!tiled) {
-    const unsigned gx = static_cast<unsigned>((a.n + 15) / 16);
-    if (a.m <= 16) hipLaunchKernelGGL((matmul_rows_kernel<O, kExact, 1, 8, 4>), dim3(gx, 1), dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((matmul_rows_kernel<O, kExact, 2, 8, 2>), dim3(gx, static_cast<unsigned>((a.m + 31) / 32)), dim3(512), 0, stream, a);
+    if constexpr (kExact) {  // 32 columns to a block halve what is read of A, where that leaves a block for most CUs
+      if (a.n > 6144) {
+        if (a.m <= 32) launch_rows<O, kExact, 2, 2, 8, 1>(a, stream);
+        else launch_rows<O, kExact, 4, 2, 8, 1>(a, stream);
+        return;
+      }
+    }
+    if (a.m <= 16) launch_rows<O, kExact, 1, 1, 8, 4>(a, stream);
+    else if (a.m <= 32) launch_rows<O, kExact, 2, 1, 8, 1>(a, stream);
+    else launch_rows<O, kExact, 4, 1, 8, 1>(a, stream);
     return;
   }
-  const size_t big_m = (a.m + 255) / 256, big_n = (a.n + 255) / 256;
-  if constexpr (!kExact) {
-    if (big_m * big_n >= 192 && a.k >= kScaleBlock) {
-      hipLaunchKernelGGL(matmul_big_kernel<O>, dim3(static_cast<unsigned>(big_m * big_n)), dim3(512), 0, stream, a,
-                         static_cast<unsigned>(big_m), static_cast<unsigned>(big_n));
-      return;
-    }
-  }
+  const Tiles split(a, 64, 64), mid(a, 128, 128), tall(a, 256, 128), big(a, 256, 256);
+  const size_t steps = (a.k + kScaleBlock - 1) / kScaleBlock, shared = (steps + kSplit - 1) / kSplit;
   if constexpr (kExact) {
-    launch_stage<O, true, 256, 128, 3>(a, stream);
+    if (split.time(1.0, 2.3, shared) < tall.time(5.0, 2.35, steps))
+      hipLaunchKernelGGL((matmul_split_kernel<O, true>), split.grid(), dim3(kSplit * 64), 0, stream, a, split.m, split.n);
+    else launch_stage<O, true, 256, 128, 3>(a, stream);
   } else {
-    if (a.m <= 64) launch_stage<O, false, 64, 128, 4>(a, stream);
-    else launch_stage<O, false, 128, 128, 4>(a, stream);
+    const double by_split = split.time(1.5, 1.05, shared), by_mid = mid.time(5.0, 0.62, steps);
+    const double by_tall = tall.time(5.0, 1.07, steps), by_big = big.time(6.0, 1.9, steps);
+    if (by_split <= std::min({by_mid, by_tall, by_big}))
+      hipLaunchKernelGGL((matmul_split_kernel<O, false>), split.grid(), dim3(kSplit * 64), 0, stream, a, split.m, split.n);
+    else if (by_mid <= std::min(by_tall, by_big)) launch_stage<O, false, 128, 128, 4>(a, stream);
+    else if (by_tall <= by_big) launch_stage<O, false, 256, 128, 3>(a, stream);
+    else hipLaunchKernelGGL(matmul_big_kernel<O>, big.grid(), dim3(512), 0, stream, a, big.m, big.n);
   }
 }
 

@@ -93,7 +93,6 @@ def test_rounding_at_every_border(fp8):
     x = np.zeros((8, 128), dtype=np.float32)
     x[:, 0] = 448.0
     x[:, 1:].flat[: v.size] = v
-    assert v.size <= 8 * 127 or True
     x = np.concatenate([x, np.pad(v, (0, -v.size % 127)).reshape(-1, 127) @ np.eye(127, 128, 1, dtype=np.float32)])
     x[8:, 0] = 448.0
     q, s = fp8.quantize(torch.from_numpy(x).cuda())
@@ -286,7 +285,7 @@ def test_norm_backward_against_differences(fp8):
 # ---- product --------------------------------------------------------------------------------
 
 
-SIZES = [(1, 1, 1), (1, 16, 128), (1, 4096, 512), (2, 130, 300), (7, 100, 1000), (16, 64, 127), (17, 129, 129), (33, 257, 640),
+SIZES = [(8, 6150, 200), (20, 6400, 1100), (40, 6200, 130), (64, 700, 3000), (70, 64, 512), (97, 450, 2049), (1, 1, 1), (1, 16, 128), (1, 4096, 512), (2, 130, 300), (7, 100, 1000), (16, 64, 127), (17, 129, 129), (33, 257, 640),
          (64, 64, 64), (65, 300, 4100), (128, 128, 128), (129, 1, 257), (200, 333, 17), (256, 256, 256), (300, 520, 1030),
          (513, 257, 384), (1, 7, 20000), (31, 40, 9000)]
 
@@ -314,10 +313,55 @@ def test_matmul_of_many_tiles_matches_the_oracle(fp8, m, n, k, tiles):
     assert (out[m:] == 7).all() and (out[:, :3] == 7).all() and (out[:, 3 + n:] == 7).all()
 
 
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("m,n,k", [(1100, 1190, 513), (1990, 2003, 300), (2050, 1921, 1024), (2100, 2113, 640), (2177, 2050, 1029)])
+def test_matmul_of_some_tiles_matches_the_oracle(fp8, m, n, k, tiles, out):
+    """Between few rows and many tiles, cut off at every side; NaN and the largest scale behind the operands."""
+    a, a64 = operand(fp8, m + k, m, k)
+    b, b64 = operand(fp8, n + 2 * k, n, k, tiles=tiles)
+
+    def buried(q):
+        rows, ld, blocks = q.values.shape[0], -(-k // 16) * 16 + 16, q.scales.shape[1]
+        v = torch.full((rows + 3, ld), 0x7F, dtype=torch.uint8, device="cuda")
+        v[:rows, :k] = q.values.view(torch.uint8)
+        s = torch.full((blocks + 1, -(-q.scales.shape[0] // 4) * 4 + 4), 255, dtype=torch.uint8, device="cuda")
+        s[:blocks, :q.scales.shape[0]] = q.scales.view(torch.uint8).t()
+        return fp8.Quantized(v.view(torch.float8_e4m3fn)[:rows, :k], s.view(torch.float8_e8m0fnu).t()[:q.scales.shape[0], :blocks])
+
+    c = torch.full((m + 1, n + 8), 7.0, dtype=out, device="cuda")
+    got = fp8.matmul(buried(a), buried(b), out=c[:m, 3:3 + n])
+    check_product(got, a64, b64, k)
+    assert (c[m:] == 7).all() and (c[:, :3] == 7).all() and (c[:, 3 + n:] == 7).all()
+    assert torch.equal(fp8.matmul(a, b, dtype=out), got)
+    a.values.view(torch.uint8)[m - 2, k - 1] = 0x7F
+    b.scales.view(torch.uint8)[-1, -1] = 255
+    if not tiles:
+        bad = fp8.matmul(a, b, dtype=out).isnan()
+        assert bad[m - 2].all() and bad[:, n - 1].all() and bad.sum() == m + n - 1
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(2000, 2000), (2100, 2100), (3600, 3600)])
+def test_matmul_of_more_tiles_at_the_ends_of_the_scales(fp8, m, n, out):
+    a, _ = operand(fp8, 1, m, 300)
+    b, _ = operand(fp8, 2, n, 300)
+    a.values.view(torch.uint8).fill_(0x38)  # ones
+    b.values.view(torch.uint8).fill_(0x38)
+    for sa, sb, want in ((0, 254, 300.0), (254, 0, 300.0), (0, 200, 300.0 * 2.0 ** -54), (254, 127, np.inf), (27, 227, 300.0)):
+        a.scales.view(torch.uint8).fill_(127)
+        b.scales.view(torch.uint8).fill_(127)
+        a.scales.view(torch.uint8)[1000:].fill_(sa)  # far ones in the later tiles alone
+        b.scales.view(torch.uint8)[900:].fill_(sb)
+        c = host(fp8.matmul(a, b, dtype=out))
+        want = host(torch.tensor([want]).to(out))
+        assert (c[:1000, :900] == host(torch.tensor([300.0]).to(out))).all() and (c[1000:, 900:] == want).all(), (sa, sb)
+
+
 def test_matmul_of_whole_numbers_is_exact(fp8):
     """Small whole numbers: every product and sum is a 32-bit value, so nothing may be off."""
     rng = np.random.default_rng(5)
-    for m, n, k in ((3, 200, 1000), (300, 270, 1100)):
+    for m, n, k in ((3, 200, 1000), (300, 270, 1100), (2000, 2100, 1100)):
         x, y = rng.integers(-8, 9, (m, k)), rng.integers(-8, 9, (n, k))
         a, b = (fp8.quantize(torch.from_numpy(z).float().cuda()) for z in (x, y))
         np.testing.assert_array_equal(host(fp8.matmul(a, b, dtype=torch.float32)), x @ y.T)
