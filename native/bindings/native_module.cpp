@@ -63,6 +63,8 @@ PYBIND11_MODULE(_tk8s_native, m) {
         py::arg("seed") = 0, py::arg("iters") = 10, py::arg("device") = 0, G());
   m.def("copy_probe", &tk8s::copy_probe, py::arg("src_device"), py::arg("dst_device"),
         py::arg("bytes"), py::arg("iters") = 10, py::arg("dma") = true, G());
+  m.def("layer_probe", &tk8s::layer_probe, py::arg("rows") = 4096, py::arg("width") = 4096, py::arg("seed") = 0,
+        py::arg("iters") = 3, py::arg("device") = 0, G());
   m.def(
       "rccl_allreduce",
       [](const std::vector<int>& devices, size_t min_bytes, size_t max_bytes, int factor,
@@ -108,6 +110,10 @@ PYBIND11_MODULE(_tk8s_native, m) {
         tk8s::philox_fill(ptr<void>(dst), nbytes, seed, stream_of(s));
       },
       py::arg("dst"), py::arg("nbytes"), py::arg("seed"), py::arg("stream") = 0);
+  m.def(
+      "layer_fill",
+      [](uintptr_t dst, size_t count, uint64_t seed, uintptr_t s) { tk8s::layer_fill(ptr<void>(dst), count, seed, stream_of(s)); },
+      py::arg("dst"), py::arg("count"), py::arg("seed"), py::arg("stream") = 0);
   m.def("md5_tree_workspace", &tk8s::md5_tree_workspace, py::arg("nbytes"),
         py::arg("chunk_bytes") = 1024);
   m.def(

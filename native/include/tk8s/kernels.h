@@ -157,4 +157,8 @@ struct MatmulArgs {
 };
 void fp8_matmul(const MatmulArgs& a, LayerType out, hipStream_t stream);
 
+// dst[i], 16-bit (kBF16): a multiple of 1/32 in [-4, 4) that depends on the seed and i alone (count a
+// multiple of 8): what the layer probe works on.
+void layer_fill(void* dst, size_t count, uint64_t seed, hipStream_t stream);
+
 }  // namespace tk8s

@@ -30,6 +30,14 @@ std::string md5_probe(size_t bytes, uint32_t chunk_bytes, uint64_t seed, int ite
 // dma: also time the SDMA-engine path (hipMemcpyPeerAsync) for a peer copy.
 std::string copy_probe(int src_device, int dst_device, size_t bytes, int iters, bool dma = true);
 
+// Matrix cores: one step of an 8-bit layer, forward and backward, on rows x width activations and a
+// width x width weight (multiples of 128, up to 16384) made from the seed: a norm after a residual, rounding to
+// 8 bits, y = x W^T, the gradients of x and W, and the norm's. Sampled rows are computed again on the
+// host in 64 bits ("error": the largest, as a share of what rounding allows; above 1 is a failure), and
+// the MD5 tree of everything that came out ("digest") has to be the same in each of the `iters` steps;
+// so must it be on every device. Reports the products' TFLOP/s and the other kernels' GB/s.
+std::string layer_probe(size_t rows, size_t width, uint64_t seed, int iters, int device);
+
 // The local probes share one grow-on-demand device allocation per device (see probes.cpp);
 // free them (e.g. from a long-lived process once validation is done).
 void release_probe_scratch();

@@ -603,6 +603,24 @@ template <class T> void launch_quantize(const QuantizeArgs& a, hipStream_t strea
   TK8S_HIP_CHECK(hipGetLastError());
 }
 
+// 8 values a thread, each of 8 bits of a 64-bit mix of their number (splitmix64's finaliser, by S. Vigna).
+__global__ __launch_bounds__(256) void layer_fill_kernel(uint4* dst, size_t eights, uint64_t seed) {
+  for (size_t i = blockIdx.x * size_t(256) + threadIdx.x; i < eights; i += static_cast<size_t>(gridDim.x) * 256) {
+    uint64_t z = (seed + 1) * 0x9e3779b97f4a7c15ull + i * 0xd1342543de82ef95ull;
+    z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+    z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+    z ^= z >> 31;
+    unsigned v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float lo = static_cast<float>(static_cast<int>(z >> (16 * j) & 255u) - 128) * (1.f / 32);
+      const float hi = static_cast<float>(static_cast<int>(z >> (16 * j + 8) & 255u) - 128) * (1.f / 32);
+      v[j] = __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xffff0000u);  // 8 significant bits: exact
+    }
+    dst[i] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+
 void check(bool ok, const char* what) {
   if (!ok) throw std::invalid_argument(what);
 }
@@ -663,6 +681,15 @@ void fp8_quantize(const QuantizeArgs& a, LayerType type, hipStream_t stream) {
     case LayerType::kBF16: return launch_quantize<__bf16>(a, stream);
     case LayerType::kF16: return launch_quantize<_Float16>(a, stream);
   }
+}
+
+void layer_fill(void* dst, size_t count, uint64_t seed, hipStream_t stream) {
+  check(count % 8 == 0, "layer_fill: the number of values must be a multiple of 8");
+  if (count == 0) return;
+  const size_t blocks = (count / 8 + 255) / 256;
+  hipLaunchKernelGGL(layer_fill_kernel, dim3(static_cast<unsigned>(std::min<size_t>(blocks, static_cast<size_t>(streaming_grid())))), dim3(256), 0,
+                     stream, static_cast<uint4*>(dst), count / 8, seed);
+  TK8S_HIP_CHECK(hipGetLastError());
 }
 
 }  // namespace tk8s

@@ -5,12 +5,17 @@
 //   tk8s-probe [--device D | --all-devices] [--gpuinfo] [--peers] [--hbm-bytes B]
 //              [--md5-bytes B] [--chunk C] [--seed S] [--copy-bytes B] [--peer-bytes B] [--no-peer-dma]
 //              [--iters K] [--mode plain|nontemporal] [--skip-md5]
+//              [--layer] [--layer-rows R] [--layer-width W]
 //              [--out FILE] [--reuse FILE [--reuse-wait S]]
 //
 // --all-devices probes every visible GPU concurrently, one host thread per device (a node with
 // k GPUs validates in the time of one). --peers then pulls --peer-bytes from every other GPU
 // into each GPU over xGMI (each destination thread walks its sources in turn, so at most one
 // transfer per destination is in flight). Exit 0 iff every probe passed.
+//
+// --layer adds the matrix cores: a step of an 8-bit layer, forward and backward, on R x W activations
+// (4096 x 4096) and a W x W weight, checked against the host and for the same bits in every step; every
+// device must come to the digest of the majority.
 //
 // Pipelined validation (node bring-up): `--out FILE` is the early burn-in started while the
 // control plane comes up; it writes the JSON atomically (FILE.tmp -> FILE) and removes the
@@ -61,12 +66,24 @@ double ms_since(std::chrono::steady_clock::time_point t) {
 }
 
 struct DeviceResult {
-  std::string hbm, md5, copy, digest;
+  std::string hbm, md5, copy, digest, layer, layer_digest;
   std::vector<std::string> peers;
-  double wall_ms = 0, hbm_ms = 0, md5_ms = 0, copy_ms = 0, peers_ms = 0;  // host wall clock per phase
+  double wall_ms = 0, hbm_ms = 0, md5_ms = 0, copy_ms = 0, layer_ms = 0, peers_ms = 0;  // host wall clock per phase
   bool ok = true;
   bool peers_ok = true;  // the links into this device: judged by xgmi.py, not part of `ok`
 };
+
+// The digest most devices came to (the first of those that tie), empty if none came to any.
+std::string majority(const std::vector<DeviceResult>& res, std::string DeviceResult::*digest) {
+  std::string want;
+  size_t best = 0;
+  for (const auto& r : res) {
+    size_t votes = 0;
+    for (const auto& o : res) votes += !(o.*digest).empty() && o.*digest == r.*digest;
+    if (votes > best) best = votes, want = r.*digest;
+  }
+  return want;
+}
 
 void emit(const std::string& json, const std::string& out_file) {
   if (!out_file.empty()) {
@@ -101,6 +118,8 @@ int main(int argc, char** argv) {
     const size_t peer_bytes = static_cast<size_t>(a.num("peer-bytes", 64LL << 20));
     const auto chunk = static_cast<uint32_t>(a.num("chunk", 1024));
     const auto seed = static_cast<uint64_t>(a.num("seed", 0));
+    const bool layer = a.has("layer");
+    const auto layer_rows = static_cast<size_t>(a.num("layer-rows", 4096)), layer_width = static_cast<size_t>(a.num("layer-width", 4096));
     const int iters = static_cast<int>(a.num("iters", 5));
     const auto mode = a.str("mode", "plain") == "nontemporal" ? tk8s::StoreMode::kNonTemporal
                                                               : tk8s::StoreMode::kPlain;
@@ -147,7 +166,13 @@ int main(int argc, char** argv) {
       t = std::chrono::steady_clock::now();
       if (copy) r.copy = tk8s::copy_probe(dev, dev, copy, iters);
       r.copy_ms = ms_since(t);
-      r.ok = ok_of(r.hbm) && (r.md5.empty() || ok_of(r.md5)) && (r.copy.empty() || ok_of(r.copy));
+      t = std::chrono::steady_clock::now();
+      if (layer) {
+        r.layer = tk8s::layer_probe(layer_rows, layer_width, seed, iters, dev);
+        r.layer_digest = field(r.layer, "digest");
+      }
+      r.layer_ms = ms_since(t);
+      r.ok = (r.layer.empty() || ok_of(r.layer)) && ok_of(r.hbm) && (r.md5.empty() || ok_of(r.md5)) && (r.copy.empty() || ok_of(r.copy));
       t = std::chrono::steady_clock::now();
       if (a.has("peers"))
         // Offset order: device k pulls from k+1, k+2, ... (mod m), so at any moment the devices
@@ -182,25 +207,23 @@ int main(int argc, char** argv) {
     if (pinned) {
       want = kKnownDigest256M;
     } else if (md5) {
-      size_t best = 0;
-      for (size_t k = 0; k < res.size(); ++k) {
-        size_t votes = 0;
-        for (const auto& o : res) votes += (!o.digest.empty() && o.digest == res[k].digest);
-        if (votes > best) best = votes, want = res[k].digest;
-      }
+      want = majority(res, &DeviceResult::digest);
     }
+    const std::string want_layer = majority(res, &DeviceResult::layer_digest);
     const bool unpinned_single = md5 && !pinned && res.size() == 1;
     bool ok = true;
     std::vector<std::string> per_dev;
     for (size_t k = 0; k < res.size(); ++k) {
       DeviceResult& r = res[k];
       const bool digest_ok = !md5 || (!r.digest.empty() && r.digest == want);
-      r.ok = r.ok && digest_ok;
+      const bool layer_ok = !layer || (!r.layer_digest.empty() && r.layer_digest == want_layer);
+      r.ok = r.ok && digest_ok && layer_ok;
       ok = ok && r.ok;
       tk8s::Json d;
-      d.kv("device", devices[k]).kv("ok", r.ok).kv("wall_ms", r.wall_ms)
-          .raw("phase_ms", tk8s::Json().kv("hbm", r.hbm_ms).kv("md5", r.md5_ms).kv("copy", r.copy_ms)
-                               .kv("peers", r.peers_ms).str())
+      tk8s::Json phases;
+      phases.kv("hbm", r.hbm_ms).kv("md5", r.md5_ms).kv("copy", r.copy_ms).kv("peers", r.peers_ms);
+      if (layer) phases.kv("layer", r.layer_ms);
+      d.kv("device", devices[k]).kv("ok", r.ok).kv("wall_ms", r.wall_ms).raw("phase_ms", phases.str())
           .raw("hbm", r.hbm);
       if (md5) {
         d.raw("md5", r.md5);
@@ -208,6 +231,11 @@ int main(int argc, char** argv) {
         else d.kv("digest_ok", digest_ok);
       }
       if (copy) d.raw("copy", r.copy);
+      if (layer) {
+        d.raw("layer", r.layer);
+        if (res.size() == 1) d.kv("layer_digest_ok", "unpinned");
+        else d.kv("layer_digest_ok", layer_ok);
+      }
       if (!r.peers.empty()) d.raw("peers", tk8s::Json::array(r.peers)).kv("peers_ok", r.peers_ok);
       per_dev.push_back(d.str());
     }
@@ -218,6 +246,7 @@ int main(int argc, char** argv) {
     out.raw("hbm", res[0].hbm);
     if (md5) out.raw("md5", res[0].md5).kv("md5_expected", want).kv("md5_pinned", pinned);
     if (copy) out.raw("copy", res[0].copy);
+    if (layer) out.raw("layer", res[0].layer).kv("layer_expected", want_layer);
     out.raw("devices", tk8s::Json::array(per_dev));
     if (!info.empty()) out.raw("gpuinfo", info);
     out.raw("timings_ms", tk8s::Json().kv("hip_init", init_ms).kv("gpuinfo", gpuinfo_ms).kv("total", ms_since(t0))

@@ -152,12 +152,17 @@ def test_native_launchers_refuse_before_launching(nat):
     with pytest.raises(ValueError, match="weight is of"):
         nat.rms_norm_fp8(4096, 16, 0, 0, 4096, 0, 0, none, 0, 0, 0, 1, 16, 1e-6, 0, 1)
     with pytest.raises(ValueError, match="pointer is missing"):
-        nat.rms_norm_backward(4096, 16, 4096, 16, 4096, 4096, 0, 0, 4096, 16, 4096, 0, 1, 16, 0, 0)
+        nat.rms_norm_backward(4096, 16, 4096, 16, 4096, 4096, 0, 0, 0, 16, 4096, 4096, 1, 16, 0, 0)
+    assert nat.rms_norm_backward_workspace(1000, 16) > 0  # where one is needed, it is missed
+    with pytest.raises(ValueError, match="pointer is missing"):
+        nat.rms_norm_backward(4096, 16, 4096, 16, 4096, 4096, 0, 0, 4096, 16, 4096, 0, 1000, 16, 0, 0)
     with pytest.raises(ValueError, match="no rows"):
         nat.rms_norm_backward(4096, 16, 4096, 16, 4096, 4096, 0, 0, 4096, 16, 4096, 4096, 0, 16, 0, 0)
     with pytest.raises(ValueError, match="c is needed"):
         nat.fp8_matmul(none, none, False, 0, 1, 1, 1, 1, 0)
     with pytest.raises(ValueError, match="pointer is missing"):
         nat.fp8_matmul(none, none, False, 4096, 1, 1, 1, 1, 0)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        nat.layer_fill(4096, 12, 0)
     with pytest.raises(ValueError, match="16-byte"):
         nat.fp8_matmul((4096, 17, 4096, 16), (4096, 16, 4096, 16), False, 4096, 1, 1, 1, 1, 0)

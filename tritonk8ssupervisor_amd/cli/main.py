@@ -44,7 +44,7 @@ def cmd_setup(args) -> int:
               validate=not args.no_validate, rccl=(None if args.rccl is None else args.rccl == "on"),
               quiet_ansible=not args.verbose, backend=args.backend, master_port=args.port,
               hbm_bytes=args.hbm_bytes, md5_bytes=args.md5_bytes, probe_iters=args.probe_iters,
-              node_grace=args.node_grace, rocprof=args.rocprof, rocprof_counters=args.rocprof_counters,
+              layer=args.layer, node_grace=args.node_grace, rocprof=args.rocprof, rocprof_counters=args.rocprof_counters,
               rccl_max_bytes=args.rccl_max_bytes,
               rccl_timeout=args.rccl_timeout, rccl_op_timeout=args.rccl_op_timeout, platform=args.platform)
     try:
@@ -360,6 +360,8 @@ SETUP_OPTIONS: list[tuple[tuple[str, ...], dict]] = [
     (("--hbm-bytes",), {"type": int, "default": 1 << 30}),
     (("--md5-bytes",), {"type": int, "default": 256 << 20}),
     (("--probe-iters",), {"type": int, "default": 3}),
+    (("--layer",), {"action": "store_true",
+                    "help": "validate the matrix cores too: a step of an 8-bit layer, forward and backward, on every GPU"}),
     (("--node-grace",), {"type": float, "default": 5.0}),
     (("--rocprof",), {"action": "store_true",
                       "help": "run the RCCL Job's ranks under rocprofv3 --kernel-trace --stats (rocprof/<job>/)"}),

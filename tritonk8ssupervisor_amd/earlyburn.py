@@ -97,13 +97,15 @@ def hsa_peers_failed(environ=None) -> bool:
 
 
 def default_validation_command(hbm_bytes: int = 1 << 30, md5_bytes: int = 256 << 20, iters: int = 3,
-                               peers: bool = True) -> list[str]:
+                               peers: bool = True, layer: bool = False) -> list[str]:
     """The validation DaemonSet payload (and the burn-in): every GPU of a worker; ``peers``: also
-    the xGMI pulls between them (workers of more than one GPU)."""
+    the xGMI pulls between them (workers of more than one GPU); ``layer``: also the matrix cores, a
+    step of an 8-bit layer forward and backward (``tk8s-probe`` only)."""
     if os.environ.get("TK8S_FAKE_GPUS"):
         return [sys.executable, "-m", "tritonk8ssupervisor_amd.ops.fakeprobe"]
-    return [probe_tool(peers), "--all-devices", "--gpuinfo", *(["--peers"] if peers else []), "--hbm-bytes",
-            str(hbm_bytes), "--md5-bytes", str(md5_bytes), "--iters", str(iters)]
+    return [os.path.join(BIN, "tk8s-probe") if layer else probe_tool(peers), "--all-devices", "--gpuinfo",
+            *(["--peers"] if peers else []), "--hbm-bytes", str(hbm_bytes), "--md5-bytes", str(md5_bytes),
+            "--iters", str(iters), *(["--layer"] if layer else [])]
 
 
 PEER_CHECK_BYTES = 16 << 20  # the Ready path's pull per link: ~0.25 ms at xGMI rates
@@ -118,7 +120,7 @@ def host_burnin_command(command: list[str], gpus: list[int]) -> list[str]:
     if len(gpus) > 1 and "--peers" not in cmd:
         cmd.append("--peers")
         tool = probe_tool(peers=True)
-        if cmd and os.path.basename(cmd[0]) != os.path.basename(tool) and \
+        if cmd and "--layer" not in cmd and os.path.basename(cmd[0]) != os.path.basename(tool) and \
                 os.path.basename(cmd[0]) in ("tk8s-hsaprobe", "tk8s-probe"):
             cmd[0] = tool  # the pulls' runtime (probe_tool)
     if "--peers" in cmd and "--peer-bytes" not in cmd:

@@ -77,13 +77,15 @@ def playbook_extra_vars(ws: Workspace, cfg: ClusterConfig, machines: dict[str, M
 
 # ---- setup ---------------------------------------------------------------------------------
 class Setup(KubeadmPlatform, FabricCheck):
+    layer = False  # validate the matrix cores too (tk8s-probe --layer)
+
     def __init__(self, ws: Workspace, *, answers: dict | None = None, assume_yes: bool = False,
                  resume: bool = False, timeout: float = 600.0, validate: bool = True, rccl: bool | None = None,
                  out: Callable[[str], None] = None, quiet_ansible: bool = True, hbm_bytes: int = 1 << 30,
                  md5_bytes: int = 256 << 20, probe_iters: int = 3, rccl_max_bytes: int = 64 << 20,
                  node_grace: float = 5.0, backend: str | None = None, master_port: int | None = None,
                  rocprof: bool = False, rccl_timeout: float | None = None, rocprof_counters: str | None = None,
-                 platform: str | None = None, rccl_op_timeout: float = 20.0):
+                 platform: str | None = None, rccl_op_timeout: float = 20.0, layer: bool = False):
         self.ws = ws
         self.answers = answers
         self.assume_yes = assume_yes
@@ -94,6 +96,7 @@ class Setup(KubeadmPlatform, FabricCheck):
         self.out = out or _flush_print
         self.quiet_ansible = quiet_ansible
         self.hbm_bytes, self.md5_bytes, self.probe_iters = hbm_bytes, md5_bytes, probe_iters
+        self.layer = layer
         self.rccl_max_bytes = rccl_max_bytes
         self.node_grace = node_grace
         self.backend = backend or os.environ.get("TK8S_BACKEND", "local")
@@ -377,7 +380,7 @@ class Setup(KubeadmPlatform, FabricCheck):
             peers = int(self.provider.package_by_id_or_name(self.cfg.HOST_PACKAGE).gpus or 0) > 1
         except Exception:  # noqa: BLE001 - no configuration yet: the full check
             pass
-        return default_validation_command(self.hbm_bytes, self.md5_bytes, self.probe_iters, peers=peers)
+        return default_validation_command(self.hbm_bytes, self.md5_bytes, self.probe_iters, peers=peers, layer=self.layer)
 
     def ansible(self) -> None:
         from .playbook import Playbook
