@@ -1006,19 +1006,19 @@ template <class O, bool kExact, int MT, int NT, int WAVES, int kAhead> void laun
 
 // Which tile makes a product: each kernel has one block on a CU at a time, so it takes
 // ceil(tiles / 256) rounds, each of a start and an end and a time for every 128 k. The figures in launch() are
-// microseconds measured on whole rounds; 16-bit products of k = 4096 with n = 4096 (and a few others):
+// microseconds measured on whole rounds. 16-bit products, microseconds:
 //
-//     m x n x k          64 x 64 (k shared)   128 x 128   256 x 128   256 x 256
-//     100 x 8192 x 2048        7.9                -           -           -      (rows kernel 16.5)
-//     256 x 4096 x 4096       12.1              19.8        29.8        50.7
-//     500 x 500 x 8000        17.7              33.1          -           -      (rows kernel 24.3)
-//     512 x 4096 x 4096       20.4              21.0        31.3        51.3
-//     2000 x 2000 x 2000      31.5              21.3        26.1        36.7
-//     1024 x 4096 x 4096      38.4              24.6        33.4        53.3
-//     777 x 5003 x 4432       57.6              47.6        39.5        58.1
-//     2048 x 4096 x 4096      74.0              50.5        39.4        57.2
-//     8192 x 1024 x 8192     132.5             104.2        74.0        97.4
-//     4096 x 4096 x 4096        -               110          85          69.3
+//     m x n x k          64 x 64 (k shared)   128 x 128   192 x 128   256 x 128   256 x 256
+//     100 x 8192 x 2048        7.9                -           -           -           -      (rows kernel 16.5)
+//     256 x 4096 x 4096       12.1              19.8        27.3        29.8        50.7
+//     500 x 500 x 8000        17.7              33.1          -           -           -      (rows kernel 24.3)
+//     512 x 4096 x 4096       20.4              21.0        28.6        31.3        51.3
+//     2000 x 2000 x 2000      31.5              21.3        24.5        26.1        36.7
+//     1024 x 4096 x 4096      38.4              24.6        31.6        33.4        53.3
+//     777 x 5003 x 4432       57.6              47.6        36.1        39.5        58.1
+//     2048 x 4096 x 4096      74.0              50.5        58.7        39.4        57.2
+//     8192 x 1024 x 8192     132.5             104.2       109.1        74.0        97.4
+//     4096 x 4096 x 4096        -               110         111          85          69.3
 //
 // and float32 ones, 64 x 64 against 256 x 128: 100 x 4096 x 4096 19.6 and 49.3, 1000 x 1000 x 8000 36.4 and
 // 96.9, 1024 x 4096 x 4096 78.3 and 61.2, 2048 x 4096 x 4096 152.5 and 79.9.
@@ -1050,7 +1050,7 @@ template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t str
     else launch_rows<O, kExact, 4, 1, 8, 1>(a, stream);
     return;
   }
-  const Tiles split(a, 64, 64), mid(a, 128, 128), tall(a, 256, 128), big(a, 256, 256);
+  const Tiles split(a, 64, 64), mid(a, 128, 128), high(a, 192, 128), tall(a, 256, 128), big(a, 256, 256);
   const size_t steps = (a.k + kScaleBlock - 1) / kScaleBlock, shared = (steps + kSplit - 1) / kSplit;
   if constexpr (kExact) {
     if (split.time(1.0, 2.3, shared) < tall.time(5.0, 2.35, steps))
@@ -1058,10 +1058,11 @@ template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t str
     else launch_stage<O, true, 256, 128, 3>(a, stream);
   } else {
     const double by_split = split.time(1.5, 1.05, shared), by_mid = mid.time(5.0, 0.62, steps);
-    const double by_tall = tall.time(5.0, 1.07, steps), by_big = big.time(6.0, 1.9, steps);
-    if (by_split <= std::min({by_mid, by_tall, by_big}))
+    const double by_high = high.time(5.0, 0.88, steps), by_tall = tall.time(5.0, 1.07, steps), by_big = big.time(6.0, 1.9, steps);
+    if (by_split <= std::min({by_mid, by_high, by_tall, by_big}))
       hipLaunchKernelGGL((matmul_split_kernel<O, false>), split.grid(), dim3(kSplit * 64), 0, stream, a, split.m, split.n);
-    else if (by_mid <= std::min(by_tall, by_big)) launch_stage<O, false, 128, 128, 4>(a, stream);
+    else if (by_mid <= std::min({by_high, by_tall, by_big})) launch_stage<O, false, 128, 128, 4>(a, stream);
+    else if (by_high <= std::min(by_tall, by_big)) launch_stage<O, false, 192, 128, 3>(a, stream);
     else if (by_tall <= by_big) launch_stage<O, false, 256, 128, 3>(a, stream);
     else hipLaunchKernelGGL(matmul_big_kernel<O>, big.grid(), dim3(512), 0, stream, a, big.m, big.n);
   }
