@@ -187,27 +187,33 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
 }
 
 template <class T, class W, bool kWhole> void launch_norm(const NormArgs& a, hipStream_t stream) {
-  auto go = [&](auto kernel, int threads, int rows_per_block) {
+  // per_cu: blocks a CU holds. More of them would hide more, but each loads the weight for fewer rows: 4 of 256
+  // threads against 8 take 10.3 us and 11.8 for 1031 x 5003 (16-bit, no residual), 24.2 and 25.4 for
+  // 4096 x 4096. Rows of 8192 over 256 threads are too long a chain when there are few of them (1031 rows
+  // 16.9 us, over 1024 threads 14.4; 16384 rows 172.9 and 172.1), those of 16384 over 512 threads likewise
+  // (30.5 and 28.9; 4096 rows 88.1 and 85.5).
+  auto go = [&](auto kernel, int threads, int rows_per_block, int per_cu) {
     const size_t blocks = (a.rows + rows_per_block - 1) / rows_per_block;
-    const size_t cap = static_cast<size_t>(streaming_grid(2048 / threads));
+    const size_t cap = static_cast<size_t>(streaming_grid(per_cu));
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(std::min(blocks, cap))), dim3(threads), 0, stream, a);
   };
-  if (a.cols <= 128) go(rms_norm_kernel<T, W, 16, 1, kWhole>, 256, 16);
-  else if (a.cols <= 256) go(rms_norm_kernel<T, W, 32, 1, kWhole>, 256, 8);
-  else if (a.cols <= 512) go(rms_norm_kernel<T, W, 64, 1, kWhole>, 256, 4);
-  else if (a.cols <= 1024) go(rms_norm_kernel<T, W, 64, 2, kWhole>, 256, 4);
+  if (a.cols <= 128) go(rms_norm_kernel<T, W, 16, 1, kWhole>, 256, 16, 8);
+  else if (a.cols <= 256) go(rms_norm_kernel<T, W, 32, 1, kWhole>, 256, 8, 8);
+  else if (a.cols <= 512) go(rms_norm_kernel<T, W, 64, 1, kWhole>, 256, 4, 8);
+  else if (a.cols <= 1024) go(rms_norm_kernel<T, W, 64, 2, kWhole>, 256, 4, 4);
   else if constexpr (sizeof(T) == 2) {
-    if (a.cols <= 2048) go(rms_norm_kernel<T, W, 64, 4, kWhole>, 256, 4);
-    else if (a.cols <= 4096) go(rms_norm_kernel<T, W, 256, 2, kWhole>, 256, 1);
-    else if (a.cols <= 8192) go(rms_norm_kernel<T, W, 256, 4, kWhole>, 256, 1);
-    else if (a.cols <= 16384) go(rms_norm_kernel<T, W, 512, 4, kWhole>, 512, 1);
-    else go(rms_norm_long_kernel<T, W>, 1024, 1);
+    if (a.cols <= 2048) go(rms_norm_kernel<T, W, 64, 4, kWhole>, 256, 4, 4);
+    else if (a.cols <= 4096) go(rms_norm_kernel<T, W, 256, 2, kWhole>, 256, 1, 4);
+    else if (a.cols <= 6144) go(rms_norm_kernel<T, W, 256, 3, kWhole>, 256, 1, 4);
+    else if (a.cols <= 8192) go(rms_norm_kernel<T, W, 1024, 1, kWhole>, 1024, 1, 2);
+    else if (a.cols <= 16384) go(rms_norm_kernel<T, W, 1024, 2, kWhole>, 1024, 1, 1);
+    else go(rms_norm_long_kernel<T, W>, 1024, 1, 2);
   } else {
-    if (a.cols <= 2048) go(rms_norm_kernel<T, W, 256, 1, kWhole>, 256, 1);
-    else if (a.cols <= 4096) go(rms_norm_kernel<T, W, 512, 1, kWhole>, 512, 1);
-    else if (a.cols <= 8192) go(rms_norm_kernel<T, W, 512, 2, kWhole>, 512, 1);
-    else if (a.cols <= 16384) go(rms_norm_kernel<T, W, 1024, 2, kWhole>, 1024, 1);
-    else go(rms_norm_long_kernel<T, W>, 1024, 1);
+    if (a.cols <= 2048) go(rms_norm_kernel<T, W, 256, 1, kWhole>, 256, 1, 4);
+    else if (a.cols <= 4096) go(rms_norm_kernel<T, W, 512, 1, kWhole>, 512, 1, 2);
+    else if (a.cols <= 8192) go(rms_norm_kernel<T, W, 512, 2, kWhole>, 512, 1, 2);
+    else if (a.cols <= 16384) go(rms_norm_kernel<T, W, 1024, 2, kWhole>, 1024, 1, 1);
+    else go(rms_norm_long_kernel<T, W>, 1024, 1, 2);
   }
   TK8S_HIP_CHECK(hipGetLastError());
 }

@@ -294,7 +294,7 @@ def test_unpacked_rccl_starts_faster_on_a_real_gpu(native_build):
         pytest.skip("no GPU")
     lib = library_dir()
     if lib is None:
-        pytest.skip(native_build.get("rccl-unpacked"))
+        pytest.skip("no RCCL built from source is kept")
     tool = Path(__file__).resolve().parents[1] / "tritonk8ssupervisor_amd" / "bin" / "tk8s-rccl"
     args = [str(tool), "--ngpus", "1", "--max-bytes", str(1 << 20), "--iters", "3", "--warmup", "1"]
     out = {}

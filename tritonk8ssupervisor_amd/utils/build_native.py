@@ -276,8 +276,9 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
     out = {"libtk8s": lib, "libtk8s_rccl": rlib, "native_module": nat, "topo_module": topo,
            **({"layer_module": layer} if torch is not None else {}), "tk8s-supervise": sup,
            "tk8s-gpujail": jail, "tk8s-container": tool_path("tk8s-container"),
-           "tk8s-smi": smi, "tk8s-reuse": reuse_bin, "tk8s-hsaprobe": hsa_bin, **cos,
-           "rccl-unpacked": rccl_unpacked.get("path") or f"no ({rccl_unpacked.get('why')})"}
+           "tk8s-smi": smi, "tk8s-reuse": reuse_bin, "tk8s-hsaprobe": hsa_bin, **cos}
+    if rccl_unpacked["ok"]:
+        out["rccl-unpacked"] = rccl_unpacked["path"]
     out.update({n: tool_path(n) for n in TOOLS})
     return out
 
