@@ -19,6 +19,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "tk8s/common.h"
 #include "tk8s/fp8_device.h"
@@ -101,8 +102,10 @@ __device__ __forceinline__ u32x4 load16(const uint8_t* row, size_t k, size_t k_e
 // share them along k, wave w the blocks w, w + WAVES, ..., so the block reads whole rows in order, and
 // join their sums in LDS in the order of the waves. B and A go from memory to registers directly;
 // kAhead of a wave's blocks are on their way at any time. A is small and stays in L2, but every block
-// reads all of it, and from rows a power of two apart that is slow (27 x 8192 by 8192 columns: 17 us for
-// A alone, 14 for B alone): NT = 2 halves it.
+// reads all of it, and from rows a power of two apart that is slow (27 x 8192 by 8192 columns, 16-bit: 17 us
+// for A alone, 14 for B alone): NT = 2 halves it, and 16-bit products of more than a few rows take the
+// tiles from LDS. One row by 4096 x 4096: 5.3 us, 3.2 TB/s of weights; the latency of one round of loads
+// and of the join is what is left.
 template <class O, bool kExact, int MT, int NT, int WAVES, int kAhead>
 __global__ __launch_bounds__(WAVES * 64) void matmul_rows_kernel(MatmulArgs a) {
   __shared__ float part[WAVES][NT * MT * 256];
@@ -602,7 +605,7 @@ __global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(
 // ------------------------------------------------------------------------------------------
 // Small tiles, shared along k
 // ------------------------------------------------------------------------------------------
-// Where larger tiles would leave most of the chip idle: a block makes 64 x 64 of C, and each of its four
+// Where larger tiles would leave most of the chip idle (100 x 8192 x 8192: 17.3 us, 128 x 128 31.5): a block makes 64 x 64 of C, and each of its four
 // waves takes every fourth step of 128 k for itself -- its own two slots in LDS, filled two steps
 // ahead and waited for by count, no barrier -- with the four sums joined in LDS at the end, in order.
 constexpr int kSplit = 4;
@@ -765,6 +768,173 @@ __global__ __launch_bounds__(kSplit * 64, 1) void matmul_split_kernel(MatmulArgs
     }
     store8(c + 8 * h, left - 8 * h, v);
   }
+}
+
+// The same at 32 x 32, for few rows or few tiles (27 rows of 8192 x 8192: 13.7 us, 4.9 TB/s of weights): 32 rows of A and 32 of B lie in LDS as the 64 rows of a tile would, rows
+// 2 j and 2 j + 1 of A at places 4 j and 4 j + 1, those of B behind them. kSmallSlots steps of a wave are on
+// their way: 128 KB for a CU.
+constexpr int kSmallSlots = 4;
+constexpr int kSmallSlot = 64 * 128 + 256;
+constexpr int kSmallPitch = 36;  // floats of a row of partial sums
+
+__device__ __forceinline__ void load_lds16_each(unsigned to, const uint8_t* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+
+template <class O, bool kExact>
+__global__ __launch_bounds__(kSplit * 64, 1) void matmul_small_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kSplit * kSmallSlots * kSmallSlot];
+  static_assert(kSplit * 32 * kSmallPitch * 4 <= sizeof(lds), "the partial sums go where the steps were");
+  const int lane = threadIdx.x % 64, group = lane / 16, j16 = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  unsigned tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const size_t m0 = static_cast<size_t>(tm) * 32, n0 = static_cast<size_t>(tn) * 32;
+  const unsigned whole = static_cast<unsigned>(a.k / kScaleBlock);
+  const unsigned steps = whole > static_cast<unsigned>(wave) ? (whole - wave + kSplit - 1) / kSplit : 0;
+  uint8_t* const mine = lds + wave * kSmallSlots * kSmallSlot;
+  const unsigned lds0 = lds_address(mine);
+
+  // where this lane's part of place 8 c + lane / 8 comes from, from k = 0 on
+  const uint8_t* from[8];
+  unsigned piece[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const int r = slot_row(8 * c + lane / 8), of_tile = 2 * (r / 4) + r % 2;
+    piece[c] = 16u * ((lane % 8) ^ (r / 4 % 8));
+    from[c] = r % 4 < 2 ? a.a.values + std::min(m0 + of_tile, a.m - 1) * a.a.ld : a.b.values + std::min(n0 + of_tile, a.n - 1) * a.b.ld;
+  }
+  // scales: lanes 0-7 a dword of A's rows each, 8-15 of B's (or the one with the tile's byte); the others repeat them
+  const bool of_b = lane / 8 % 2;
+  const size_t tile_n = n0 / kScaleBlock;
+  const uint8_t* const scales = !of_b       ? a.a.scales + std::min(m0 + 4 * (lane % 8), (a.m - 1) / 4 * 4)
+                                : a.b_tiles ? a.b.scales + tile_n / 4 * 4
+                                            : a.b.scales + std::min(n0 + 4 * (lane % 8), (a.n - 1) / 4 * 4);
+  const size_t scale_step = of_b ? a.b.ld_scales : a.a.ld_scales;
+
+  constexpr int kLoads = 9;
+  auto load = [&](unsigned s, unsigned slot) {  // behind the last step it is read once more, for the counts
+    const size_t b = static_cast<size_t>(s < steps ? s : steps - 1) * kSplit + wave;
+    const unsigned to = lds0 + slot * kSmallSlot;
+    load_lds4_each(to + 64 * 128, scales + b * scale_step);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) load_lds16_each(to + c * 1024, from[c] + piece[c] + b * kScaleBlock);
+  };
+  unsigned lane_at[2][2];
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      lane_at[odd][h] = lds0 + 512u * j16 + 128u * (odd ^ (j16 / 8)) + 16u * ((4 * h + group) ^ (j16 % 8));
+  struct Step {
+    Fragment a[2], b[2];
+    unsigned sa, sb;  // bytes 0 and 1
+  };
+  const size_t row2 = m0 + 2 * j16, col2 = n0 + 2 * j16;
+  const unsigned pick = a.b_tiles ? static_cast<unsigned>(tile_n % 4) * 0x0101u : j16 % 2 ? 0x0302u : 0x0100u;
+  auto read = [&](unsigned slot, Step& f) {
+    typedef const __attribute__((address_space(3))) u32x4* lds16;
+    const unsigned* const at = reinterpret_cast<const unsigned*>(mine + slot * kSmallSlot + 64 * 128);
+    f.sa = __builtin_amdgcn_perm(0, at[j16 / 2], j16 % 2 ? 0x0302u : 0x0100u);
+    f.sb = __builtin_amdgcn_perm(0, at[8 + j16 / 2], pick);
+    if constexpr (kExact) {
+      f.sa = own_scales(f.sa, row2, a.m);
+      if (!a.b_tiles) f.sb = own_scales(f.sb, col2, a.n);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f.a[i].half[h] = *reinterpret_cast<lds16>(lane_at[i][h] + slot * kSmallSlot);
+        f.b[i].half[h] = *reinterpret_cast<lds16>(lane_at[i][h] + slot * kSmallSlot + 256);
+      }
+  };
+  f32x4 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply_all = [&](const Step& f) {
+    if constexpr (!kExact) {
+      acc[0][0] = mfma_scaled<0, 0>(f.b[0], f.a[0], acc[0][0], f.sb, f.sa);
+      acc[0][1] = mfma_scaled<1, 0>(f.b[1], f.a[0], acc[0][1], f.sb, f.sa);
+      acc[1][0] = mfma_scaled<0, 1>(f.b[0], f.a[1], acc[1][0], f.sb, f.sa);
+      acc[1][1] = mfma_scaled<1, 1>(f.b[1], f.a[1], acc[1][1], f.sb, f.sa);
+    } else {
+      const bool far = far_scale(f.sa & 255u) || far_scale(f.sa >> 8 & 255u) || far_scale(f.sb & 255u) || far_scale(f.sb >> 8 & 255u);
+      const bool near = __builtin_amdgcn_ballot_w64(far) == 0;
+      Wide wb[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) wb[j] = widen(f.b[j], near ? scale_value(f.sb >> (8 * j) & 255u) : 1.f);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Wide wa = widen(f.a[i], near ? scale_value(f.sa >> (8 * i) & 255u) : 1.f);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (near) {
+            acc[i][j] = multiply(wb[j], wa, acc[i][j]);
+          } else {
+            const f32x4 p = multiply(wb[j], wa, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              acc[i][j][r] += scaled(p[r], f.sa >> (8 * i) & 255u, __shfl(f.sb, 4 * group + r, 64) >> (8 * j) & 255u);
+          }
+        }
+      }
+    }
+  };
+
+  Step f[2];
+  if (steps) {
+#pragma unroll
+    for (int s = 0; s < kSmallSlots; ++s) load(s, s);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kSmallSlots - 1) * kLoads) : "memory");
+    read(0, f[0]);
+    auto step = [&](unsigned s, const Step& now, Step& then) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // step s is in registers: its slot is free
+      load(s + kSmallSlots, s % kSmallSlots);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kSmallSlots - 1) * kLoads) : "memory");  // step s + 1 is in LDS
+      read((s + 1) % kSmallSlots, then);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply_all(now);
+    };
+    for (unsigned s = 0; s < steps; s += 2) {
+      step(s, f[0], f[1]);
+      if (s + 1 < steps) step(s + 1, f[1], f[0]);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
+  if (a.k % kScaleBlock && whole % kSplit == static_cast<unsigned>(wave)) {  // the block cut off by the end of the rows
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      *reinterpret_cast<u32x4*>(mine + c * 1024 + lane * 16) = load16(from[c], static_cast<size_t>(whole) * kScaleBlock + piece[c], a.k);
+    load_lds4_each(lds0 + 64 * 128, scales + whole * scale_step);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    read(0, f[0]);
+    multiply_all(f[0]);
+  }
+
+  __syncthreads();  // everyone has read its last step
+  float* const part = reinterpret_cast<float*>(lds) + wave * 32 * kSmallPitch;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)  // lane: row 2 j16 + i, columns 8 group + 2 r + j
+      *reinterpret_cast<f32x4*>(part + (2 * j16 + i) * kSmallPitch + 8 * group + 4 * h) =
+          f32x4{acc[i][0][2 * h], acc[i][1][2 * h], acc[i][0][2 * h + 1], acc[i][1][2 * h + 1]};
+  __syncthreads();
+  if (wave >= 2) return;
+  const int row = threadIdx.x / 4, col = threadIdx.x % 4 * 8;
+  if (m0 + row >= a.m) return;
+  const float* const sums = reinterpret_cast<const float*>(lds) + row * kSmallPitch + col;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = sums[e];
+#pragma unroll
+    for (int w = 1; w < kSplit; ++w) v[e] += sums[w * 32 * kSmallPitch + e];
+  }
+  store8(static_cast<O*>(a.c) + (m0 + row) * a.ldc + n0 + col, a.n > n0 + col ? static_cast<int>(std::min<size_t>(a.n - n0 - col, 8)) : 0, v);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1004,24 +1174,35 @@ template <class O, bool kExact, int MT, int NT, int WAVES, int kAhead> void laun
   hipLaunchKernelGGL((matmul_rows_kernel<O, kExact, MT, NT, WAVES, kAhead>), grid, dim3(WAVES * 64), 0, stream, a);
 }
 
-// Which tile makes a product: each kernel has one block on a CU at a time, so it takes
-// ceil(tiles / 256) rounds, each of a start and an end and a time for every 128 k. The figures in launch() are
-// microseconds measured on whole rounds. 16-bit products, microseconds:
+// Which tile makes a product: each kernel has one block on a CU at a time, so it takes ceil(tiles / 256) rounds,
+// each of a start and an end and a time for every 128 k (for every 512 where four waves share k). The
+// figures in launch() are microseconds, fitted to these (those in brackets are not chosen). 16-bit:
 //
-//     m x n x k          64 x 64 (k shared)   128 x 128   192 x 128   256 x 128   256 x 256
-//     100 x 8192 x 2048        7.9                -           -           -           -      (rows kernel 16.5)
-//     256 x 4096 x 4096       12.1              19.8        27.3        29.8        50.7
-//     500 x 500 x 8000        17.7              33.1          -           -           -      (rows kernel 24.3)
-//     512 x 4096 x 4096       20.4              21.0        28.6        31.3        51.3
-//     2000 x 2000 x 2000      31.5              21.3        24.5        26.1        36.7
-//     1024 x 4096 x 4096      38.4              24.6        31.6        33.4        53.3
-//     777 x 5003 x 4432       57.6              47.6        36.1        39.5        58.1
-//     2048 x 4096 x 4096      74.0              50.5        58.7        39.4        57.2
-//     8192 x 1024 x 8192     132.5             104.2       109.1        74.0        97.4
-//     4096 x 4096 x 4096        -               110         111          85          69.3
+//     m x n x k            32 x 32   64 x 64   128 x 128   192 x 128   256 x 128   256 x 256
+//     32 x 8192 x 8192      14.2     (15.8)
+//     24 x 4096 x 4096       6.4     (9.2)                                                    (rows 8.1)
+//     16 x 1024 x 8192       8.0     (12.3)                                                   (rows 10.4)
+//     500 x 500 x 8000      10.3     (17.9)     (33.1)
+//     27 x 14336 x 4096    (14.9)     13.5                                                    (rows 23.4)
+//     100 x 8192 x 8192    (33.1)     17.3      (31.5)
+//     256 x 4096 x 4096    (23.4)     12.1      (19.8)      (27.3)      (29.8)      (50.7)
+//     512 x 4096 x 4096               20.4      (21.0)      (28.6)      (31.3)      (51.3)
+//     2000 x 2000 x 2000             (31.5)      21.3       (24.5)      (26.1)      (36.7)
+//     1024 x 4096 x 4096             (38.4)      24.6       (31.6)      (33.4)      (53.3)
+//     777 x 5003 x 4432              (57.6)     (47.6)       36.1       (39.5)      (58.1)
+//     2048 x 4096 x 4096             (74.0)     (50.5)      (58.7)       39.4       (57.2)
+//     8192 x 1024 x 8192            (132.5)    (104.2)     (109.1)       74.0       (97.4)
+//     4096 x 4096 x 4096                        (110)       (111)        (85)        69.3
 //
-// and float32 ones, 64 x 64 against 256 x 128: 100 x 4096 x 4096 19.6 and 49.3, 1000 x 1000 x 8000 36.4 and
-// 96.9, 1024 x 4096 x 4096 78.3 and 61.2, 2048 x 4096 x 4096 152.5 and 79.9.
+// float32, whose tiles wait for the widening:
+//
+//     m x n x k            32 x 32   64 x 64   256 x 128
+//     64 x 4096 x 4096      11.4     (19.3)                (rows 12.9)
+//     100 x 1024 x 8192     16.6     (30.2)                (rows 21.5)
+//     100 x 8192 x 1024    (19.9)     11.1                 (rows 11.9)
+//     1000 x 1000 x 8000              36.4      (96.9)
+//     1024 x 4096 x 4096             (78.3)      61.2
+//     2048 x 4096 x 4096            (152.5)      79.9
 struct Tiles {
   unsigned m, n;
   Tiles(const MatmulArgs& a, size_t tm, size_t tn) : m(static_cast<unsigned>((a.m + tm - 1) / tm)), n(static_cast<unsigned>((a.n + tn - 1) / tn)) {}
@@ -1033,37 +1214,37 @@ struct Tiles {
 };
 
 template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t stream) {
-  // Rows too long for the tiles' 32-bit offsets, and few rows of A: the tiles of 64 columns leave most CUs
-  // without one while n <= 6144 (16-bit, 24 x 4096 x 4096: rows 7.9 us, tiles 9.0; 64 x 4096 x 4096 13.9 and
-  // 9.1; 24 x 14336 x 4096 18.2 and 13.4), and they are slow at float32 (64 x 4096 x 4096: 13.1 and 18.9).
-  const bool tiled = a.a.ld < (1u << 23) && a.b.ld < (1u << 23) && (a.m > 64 || (!kExact && (a.m > 32 || a.n > 6144)));
-  if (!tiled) {
-    if constexpr (kExact) {  // 32 columns to a block halve what is read of A, where that leaves a block for most CUs
-      if (a.n > 6144) {
-        if (a.m <= 32) launch_rows<O, kExact, 2, 2, 8, 1>(a, stream);
-        else launch_rows<O, kExact, 4, 2, 8, 1>(a, stream);
-        return;
-      }
-    }
-    if (a.m <= 16) launch_rows<O, kExact, 1, 1, 8, 4>(a, stream);
-    else if (a.m <= 32) launch_rows<O, kExact, 2, 1, 8, 1>(a, stream);
-    else launch_rows<O, kExact, 4, 1, 8, 1>(a, stream);
-    return;
-  }
-  const Tiles split(a, 64, 64), mid(a, 128, 128), high(a, 192, 128), tall(a, 256, 128), big(a, 256, 256);
+  const Tiles small(a, 32, 32), split(a, 64, 64), mid(a, 128, 128), high(a, 192, 128), tall(a, 256, 128), big(a, 256, 256);
   const size_t steps = (a.k + kScaleBlock - 1) / kScaleBlock, shared = (steps + kSplit - 1) / kSplit;
+  auto by_small = [&] { hipLaunchKernelGGL((matmul_small_kernel<O, kExact>), small.grid(), dim3(kSplit * 64), 0, stream, a, small.m, small.n); };
+  auto by_split = [&] { hipLaunchKernelGGL((matmul_split_kernel<O, kExact>), split.grid(), dim3(kSplit * 64), 0, stream, a, split.m, split.n); };
+  // rows too long for the larger tiles' 32-bit offsets
+  if (a.a.ld >= (1u << 23) || a.b.ld >= (1u << 23)) return by_small();
   if constexpr (kExact) {
-    if (split.time(1.0, 2.3, shared) < tall.time(5.0, 2.35, steps))
-      hipLaunchKernelGGL((matmul_split_kernel<O, true>), split.grid(), dim3(kSplit * 64), 0, stream, a, split.m, split.n);
+    // Few rows of A: widened tiles wait for themselves, rows have more waves to take turns (16 x 4096 x 4096
+    // 7.8 us and 10.4; 64 x 8192 x 1024: 7.2 and 10.8, but 64 x 4096 x 4096: 12.9 and 11.4).
+    // 32 columns to a block halve what is read of A, where that leaves a block for most CUs.
+    if (a.m <= 16 && a.n <= 6144) return launch_rows<O, true, 1, 1, 8, 4>(a, stream);
+    if (a.m <= 32) return a.n <= 6144 ? launch_rows<O, true, 2, 1, 8, 1>(a, stream) : launch_rows<O, true, 2, 2, 8, 1>(a, stream);
+    if (a.m <= 64 && a.n > 6144 && a.k <= 2048) return launch_rows<O, true, 4, 2, 8, 1>(a, stream);
+    const double smalls = small.time(3.2, 0.85, shared), splits = split.time(6.0, 1.6, shared), talls = tall.time(5.0, 2.35, steps);
+    if (smalls <= std::min(splits, talls)) by_small();
+    else if (splits <= talls) by_split();
     else launch_stage<O, true, 256, 128, 3>(a, stream);
   } else {
-    const double by_split = split.time(1.5, 1.05, shared), by_mid = mid.time(5.0, 0.62, steps);
-    const double by_high = high.time(5.0, 0.88, steps), by_tall = tall.time(5.0, 1.07, steps), by_big = big.time(6.0, 1.9, steps);
-    if (by_split <= std::min({by_mid, by_high, by_tall, by_big}))
-      hipLaunchKernelGGL((matmul_split_kernel<O, false>), split.grid(), dim3(kSplit * 64), 0, stream, a, split.m, split.n);
-    else if (by_mid <= std::min({by_high, by_tall, by_big})) launch_stage<O, false, 128, 128, 4>(a, stream);
-    else if (by_high <= std::min(by_tall, by_big)) launch_stage<O, false, 192, 128, 3>(a, stream);
-    else if (by_tall <= by_big) launch_stage<O, false, 256, 128, 3>(a, stream);
+    // One token or so: 16 columns to a block put 1024 < n <= 4096 on twice as many CUs (4096 x 4096: 5.6 us and
+    // 6.2; 1024 x 8192: 7.8 both; 1000 x 1024: 5.7 and 5.2; 8192 x 1024: 7.5 and 5.3). From 8 rows on they
+    // are no faster.
+    if (a.m <= 4 && a.n > 1024 && a.n <= 4096) return launch_rows<O, false, 1, 1, 8, 4>(a, stream);
+    const double smalls = small.time(2.7, 0.45, shared), splits = split.time(4.5, 0.75, shared), mids = mid.time(5.0, 0.62, steps);
+    const double highs = high.time(5.0, 0.88, steps), talls = tall.time(5.0, 1.07, steps);
+    const double bigs = a.k >= kScaleBlock ? big.time(6.0, 1.9, steps) : HUGE_VAL;  // it takes at least one whole block
+    const double least = std::min({smalls, splits, mids, highs, talls, bigs});
+    if (least == smalls) by_small();
+    else if (least == splits) by_split();
+    else if (least == mids) launch_stage<O, false, 128, 128, 4>(a, stream);
+    else if (least == highs) launch_stage<O, false, 192, 128, 3>(a, stream);
+    else if (least == talls) launch_stage<O, false, 256, 128, 3>(a, stream);
     else hipLaunchKernelGGL(matmul_big_kernel<O>, big.grid(), dim3(512), 0, stream, a, big.m, big.n);
   }
 }

@@ -285,7 +285,7 @@ def test_norm_backward_against_differences(fp8):
 # ---- product --------------------------------------------------------------------------------
 
 
-SIZES = [(8, 6150, 200), (20, 6400, 1100), (40, 6200, 130), (64, 700, 3000), (70, 64, 512), (97, 450, 2049), (1, 1, 1), (1, 16, 128), (1, 4096, 512), (2, 130, 300), (7, 100, 1000), (16, 64, 127), (17, 129, 129), (33, 257, 640),
+SIZES = [(3, 1500, 700), (5, 9000, 260), (20, 14400, 520), (33, 4100, 1500), (130, 8200, 400), (64, 6200, 2100), (50, 6300, 1000), (8, 6150, 200), (20, 6400, 1100), (40, 6200, 130), (64, 700, 3000), (70, 64, 512), (97, 450, 2049), (1, 1, 1), (1, 16, 128), (1, 4096, 512), (2, 130, 300), (7, 100, 1000), (16, 64, 127), (17, 129, 129), (33, 257, 640),
          (64, 64, 64), (65, 300, 4100), (128, 128, 128), (129, 1, 257), (200, 333, 17), (256, 256, 256), (300, 520, 1030),
          (513, 257, 384), (1, 7, 20000), (31, 40, 9000)]
 
@@ -356,6 +356,29 @@ def test_matmul_of_more_tiles_at_the_ends_of_the_scales(fp8, m, n, out):
         c = host(fp8.matmul(a, b, dtype=out))
         want = host(torch.tensor([want]).to(out))
         assert (c[:1000, :900] == host(torch.tensor([300.0]).to(out))).all() and (c[1000:, 900:] == want).all(), (sa, sb)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_matmul_of_rows_far_apart(fp8, out):
+    """Rows 2^23 bytes apart: offsets into A pass 32 bits."""
+    m, n, k = 600, 70, 300
+    a, a64 = operand(fp8, 1, m, k)
+    b, b64 = operand(fp8, 2, n, k)
+    far = torch.empty(m, 1 << 23, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    far[:, :k].view(torch.uint8).copy_(a.values.view(torch.uint8))
+    got = fp8.matmul((far[:, :k], a.scales), b, dtype=out)
+    check_product(got, a64, b64, k)
+    check_product(fp8.matmul(b, (far[:, :k], a.scales), dtype=out), b64, a64, k)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [1, 16, 100, 127])
+def test_matmul_of_less_than_a_block(fp8, k, out):
+    """However large C is."""
+    for m, n in ((3, 2050), (600, 700), (1500, 1500), (3600, 3600)):
+        a, a64 = operand(fp8, m, m, k)
+        b, b64 = operand(fp8, n + 1, n, k)
+        check_product(fp8.matmul(a, b, dtype=out), a64, b64, k)
 
 
 def test_matmul_of_whole_numbers_is_exact(fp8):
