@@ -65,6 +65,12 @@ __device__ __forceinline__ f32x4 multiply(const Wide& b, const Wide& a, f32x4 ac
   return acc;
 }
 
+template <int OB, int OA>
+__device__ __forceinline__ f32x4 mfma_scaled(const Fragment& b, const Fragment& a, f32x4 acc, unsigned sb, unsigned sa) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, acc, 0, 0, OB, static_cast<int>(sb), OA,
+                                                          static_cast<int>(sa));
+}
+
 __device__ __forceinline__ float scale_value(unsigned byte) { return __uint_as_float(byte << 23); }
 
 // Scales that widened values can carry: products of two such, and 448 times one, are 32-bit numbers
@@ -98,98 +104,57 @@ __device__ __forceinline__ u32x4 load16(const uint8_t* row, size_t k, size_t k_e
 // ------------------------------------------------------------------------------------------
 // Few rows of A
 // ------------------------------------------------------------------------------------------
-// The weights are read once and that is what it should take. A block makes 16 NT columns of C; its waves
-// share them along k, wave w the blocks w, w + WAVES, ..., so the block reads whole rows in order, and
-// join their sums in LDS in the order of the waves. B and A go from memory to registers directly;
-// kAhead of a wave's blocks are on their way at any time. A is small and stays in L2, but every block
-// reads all of it, and from rows a power of two apart that is slow (27 x 8192 by 8192 columns, 16-bit: 17 us
-// for A alone, 14 for B alone): NT = 2 halves it, and 16-bit products of more than a few rows take the
-// tiles from LDS. One row by 4096 x 4096: 5.3 us, 3.2 TB/s of weights; the latency of one round of loads
-// and of the join is what is left.
-template <class O, bool kExact, int MT, int NT, int WAVES, int kAhead>
-__global__ __launch_bounds__(WAVES * 64) void matmul_rows_kernel(MatmulArgs a) {
-  __shared__ float part[WAVES][NT * MT * 256];
+// Up to 16. The weights are read once and that is what it should take. A block makes 16 columns of C; its
+// waves share them along k, wave w the blocks w, w + kRowWaves, ..., so the block reads whole rows in
+// order, and join their sums in LDS in the order of the waves. B and A go from memory to registers
+// directly; kAhead of a wave's blocks are on their way at any time. One row by 4096 x 4096: 5.3 us, 3.2 TB/s
+// of weights; the latency of one round of loads and of the join is what is left.
+constexpr int kRowWaves = 8, kAhead = 4;
+
+template <class O, bool kExact>
+__global__ __launch_bounds__(kRowWaves * 64) void matmul_rows_kernel(MatmulArgs a) {
+  __shared__ float part[kRowWaves][256];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, group = lane / 16;
-  const size_t n0 = static_cast<size_t>(blockIdx.x) * (16 * NT), m0 = static_cast<size_t>(blockIdx.y) * (16 * MT);
+  const size_t n0 = static_cast<size_t>(blockIdx.x) * 16;
   const size_t nb = (a.k + kScaleBlock - 1) / kScaleBlock;
   const size_t whole = a.k / kScaleBlock;  // blocks with all their values
-  const uint8_t *brow[NT], *bscale[NT], *arow[MT], *ascale[MT];  // what is behind the last row is computed, not stored
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const size_t n = std::min(n0 + 16 * j + lane % 16, a.n - 1);
-    brow[j] = a.b.values + n * a.b.ld + 16 * group;
-    bscale[j] = a.b.scales + (a.b_tiles ? n / kScaleBlock : n);
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const size_t m = std::min(m0 + 16 * i + lane % 16, a.m - 1);
-    arow[i] = a.a.values + m * a.a.ld + 16 * group;
-    ascale[i] = a.a.scales + m;
-  }
-  f32x4 acc[NT][MT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // what is behind the last row of either is computed, not stored
+  const size_t n = std::min(n0 + lane % 16, a.n - 1), m = std::min<size_t>(lane % 16, a.m - 1);
+  const uint8_t* const brow = a.b.values + n * a.b.ld;
+  const uint8_t* const arow = a.a.values + m * a.a.ld;
+  const uint8_t* const bscale = a.b.scales + (a.b_tiles ? n / kScaleBlock : n);
+  const uint8_t* const ascale = a.a.scales + m;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 
-  auto step = [&](const Fragment (&fb)[NT], const Fragment (&fa)[MT], const unsigned (&sb)[NT], const unsigned (&sa)[MT]) {
+  auto step = [&](const Fragment& fb, const Fragment& fa, unsigned sb, unsigned sa) {
     if constexpr (!kExact) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa[i].v, acc[j][i], 0, 0, 0, static_cast<int>(sb[j]), 0,
-                                                                      static_cast<int>(sa[i]));
+      acc = mfma_scaled<0, 0>(fb, fa, acc, sb, sa);
+    } else if (__builtin_amdgcn_ballot_w64(far_scale(sb) || far_scale(sa)) == 0) {
+      acc = multiply(widen(fb, scale_value(sb)), widen(fa, scale_value(sa)), acc);
     } else {
-      bool far = false;
+      const f32x4 p = multiply(widen(fb, 1.f), widen(fa, 1.f), f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-      for (int j = 0; j < NT; ++j) far = far || far_scale(sb[j]);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) far = far || far_scale(sa[i]);
-      const bool near = __builtin_amdgcn_ballot_w64(far) == 0;
-      Wide wb[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) wb[j] = widen(fb[j], near ? scale_value(sb[j]) : 1.f);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const Wide wa = widen(fa[i], near ? scale_value(sa[i]) : 1.f);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if (near) {
-            acc[j][i] = multiply(wb[j], wa, acc[j][i]);
-          } else {
-            const f32x4 p = multiply(wb[j], wa, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[j][i][r] += scaled(p[r], sa[i], __shfl(sb[j], 4 * group + r, 64));
-          }
-        }
-      }
+      for (int r = 0; r < 4; ++r) acc[r] += scaled(p[r], sa, __shfl(sb, 4 * group + r, 64));
     }
   };
 
-  // This wave's whole blocks: wave, wave + WAVES, ..., from a place of the block's own on and round, so that
-  // the blocks do not all ask the same channel of L2 for the same piece of A (27 x 8192: 22 -> 20 us).
+  // This wave's whole blocks: wave, wave + kRowWaves, ..., from a place of the block's own on and round, so that
+  // the blocks do not all ask the same channel of L2 for the same piece of A.
   // Loads come back in the order of their requests, so A's are made as early as B's, though A is near.
-  const unsigned steps = whole > static_cast<size_t>(wave) ? static_cast<unsigned>((whole - wave + WAVES - 1) / WAVES) : 0;
-  Fragment fb[kAhead][NT], fa[kAhead][MT];
-  unsigned sb[kAhead][NT], sa[kAhead][MT];
+  const unsigned steps = whole > static_cast<size_t>(wave) ? static_cast<unsigned>((whole - wave + kRowWaves - 1) / kRowWaves) : 0;
+  Fragment fb[kAhead], fa[kAhead];
+  unsigned sb[kAhead], sa[kAhead];
   const unsigned turn = steps ? blockIdx.x & ((1u << (31 - __builtin_clz(steps))) - 1) : 0;
   auto request = [&](unsigned s, int u) {
     unsigned q = (s < steps ? s : steps - 1) + turn;
     q = q >= steps ? q - steps : q;
-    const size_t at = wave + static_cast<size_t>(q) * WAVES;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      fb[u][j].half[0] = *reinterpret_cast<const u32x4*>(brow[j] + at * kScaleBlock);
-      fb[u][j].half[1] = *reinterpret_cast<const u32x4*>(brow[j] + at * kScaleBlock + 64);
-      sb[u][j] = bscale[j][at * a.b.ld_scales];
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      fa[u][i].half[0] = *reinterpret_cast<const u32x4*>(arow[i] + at * kScaleBlock);
-      fa[u][i].half[1] = *reinterpret_cast<const u32x4*>(arow[i] + at * kScaleBlock + 64);
-      sa[u][i] = ascale[i][at * a.a.ld_scales];
-    }
+    const size_t at = wave + static_cast<size_t>(q) * kRowWaves, k = at * kScaleBlock + 16 * group;
+    fb[u].half[0] = *reinterpret_cast<const u32x4*>(brow + k);
+    fb[u].half[1] = *reinterpret_cast<const u32x4*>(brow + k + 64);
+    sb[u] = bscale[at * a.b.ld_scales];
+    fa[u].half[0] = *reinterpret_cast<const u32x4*>(arow + k);
+    fa[u].half[1] = *reinterpret_cast<const u32x4*>(arow + k + 64);
+    sa[u] = ascale[at * a.a.ld_scales];
   };
   if (steps) {
 #pragma unroll
@@ -203,38 +168,26 @@ __global__ __launch_bounds__(WAVES * 64) void matmul_rows_kernel(MatmulArgs a) {
       }
     }
   }
-  const size_t b = wave + static_cast<size_t>(steps) * WAVES;
+  const size_t b = wave + static_cast<size_t>(steps) * kRowWaves;
   if (b < nb) {  // the block cut off by the end of the rows, if it is this wave's
     const size_t k = b * kScaleBlock + 16 * group;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      fb[0][j].half[0] = load16(brow[j] - 16 * group, k, a.k);
-      fb[0][j].half[1] = load16(brow[j] - 16 * group, k + 64, a.k);
-      sb[0][j] = bscale[j][b * a.b.ld_scales];
+    for (int h = 0; h < 2; ++h) {
+      fb[0].half[h] = load16(brow, k + 64 * h, a.k);
+      fa[0].half[h] = load16(arow, k + 64 * h, a.k);
     }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      fa[0][i].half[0] = load16(arow[i] - 16 * group, k, a.k);
-      fa[0][i].half[1] = load16(arow[i] - 16 * group, k + 64, a.k);
-      sa[0][i] = ascale[i][b * a.a.ld_scales];
-    }
-    step(fb[0], fa[0], sb[0], sa[0]);
+    step(fb[0], fa[0], bscale[b * a.b.ld_scales], ascale[b * a.a.ld_scales]);
   }
 
   // lane: row lane % 16 of A, columns 4 * group .. + 3
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-      *reinterpret_cast<f32x4*>(&part[wave][(j * MT + i) * 256 + (lane % 16) * 16 + 4 * group]) = acc[j][i];
+  *reinterpret_cast<f32x4*>(&part[wave][lane % 16 * 16 + 4 * group]) = acc;
   __syncthreads();
-  for (int e = threadIdx.x; e < NT * MT * 256; e += WAVES * 64) {
-    float s = part[0][e];
+  if (threadIdx.x >= 256) return;
+  float sum = part[0][threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) s += part[w][e];
-    const size_t row = m0 + e / 256 % MT * 16 + e % 256 / 16, col = n0 + e / 256 / MT * 16 + e % 16;
-    if (row < a.m && col < a.n) static_cast<O*>(a.c)[row * a.ldc + col] = static_cast<O>(s);
-  }
+  for (int w = 1; w < kRowWaves; ++w) sum += part[w][threadIdx.x];
+  const size_t row = threadIdx.x / 16, col = n0 + threadIdx.x % 16;
+  if (row < a.m && col < a.n) static_cast<O*>(a.c)[row * a.ldc + col] = static_cast<O>(sum);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -249,12 +202,6 @@ __global__ __launch_bounds__(WAVES * 64) void matmul_rows_kernel(MatmulArgs a) {
 // in the upper 32, so that of a fragment's rows 4 j + i those with j < 8 and j >= 8 lie in different
 // halves of the 64 banks.
 __device__ __forceinline__ int slot_row(int p) { return p ^ (p / 32 % 2); }
-
-template <int OB, int OA>
-__device__ __forceinline__ f32x4 mfma_scaled(const Fragment& b, const Fragment& a, f32x4 acc, unsigned sb, unsigned sa) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, acc, 0, 0, OB, static_cast<int>(sb), OA,
-                                                          static_cast<int>(sa));
-}
 
 constexpr int kXcds = 8;   // dies with an L2 of their own; blocks go to them in turn
 constexpr int kPanel = 8;  // tiles of A that a die's neighbouring blocks share
@@ -605,10 +552,10 @@ __global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(
 // ------------------------------------------------------------------------------------------
 // Small tiles, shared along k
 // ------------------------------------------------------------------------------------------
-// Where larger tiles would leave most of the chip idle (100 x 8192 x 8192: 17.3 us, 128 x 128 31.5): a block makes 64 x 64 of C, and each of its four
-// waves takes every fourth step of 128 k for itself -- its own two slots in LDS, filled two steps
-// ahead and waited for by count, no barrier -- with the four sums joined in LDS at the end, in order.
-constexpr int kSplit = 4;
+// Where larger tiles would leave most of the chip idle (100 x 8192 x 8192: 17.3 us, 128 x 128 31.5): a block makes 64 x 64
+// of C, and each of its WAVES waves takes every WAVES-th step of 128 k for itself -- its own slots in LDS,
+// eight in all, waited for by count, no barrier -- with the sums joined in LDS at the end, in
+// order. Four waves keep two steps each on their way; eight (32-bit results) one, and two to a SIMD.
 constexpr int kSplitSlot = 128 * 128 + 256;  // 64 rows of A, 64 of B, 16 dwords of scales of each (and room)
 constexpr int kSplitPitch = 68;              // floats of a row of partial sums
 
@@ -617,18 +564,19 @@ __device__ __forceinline__ void load_lds4_each(unsigned to, const uint8_t* from)
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
 }
 
-template <class O, bool kExact>
-__global__ __launch_bounds__(kSplit * 64, 1) void matmul_split_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kSplit * 2 * kSplitSlot];
-  static_assert(kSplit * 64 * kSplitPitch * 4 <= kSplit * 2 * kSplitSlot, "the partial sums go where the steps were");
+template <class O, bool kExact, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void matmul_split_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
+  constexpr int kSlots = 8 / WAVES;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[8 * kSplitSlot];
+  static_assert(4 * 64 * kSplitPitch * 4 <= sizeof(lds), "four waves' sums go where the steps were");
   const int lane = threadIdx.x % 64, group = lane / 16, j16 = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   unsigned tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
   const size_t m0 = static_cast<size_t>(tm) * 64, n0 = static_cast<size_t>(tn) * 64;
   const unsigned whole = static_cast<unsigned>(a.k / kScaleBlock);
-  const unsigned steps = whole > static_cast<unsigned>(wave) ? (whole - wave + kSplit - 1) / kSplit : 0;
-  uint8_t* const mine = lds + wave * 2 * kSplitSlot;
+  const unsigned steps = whole > static_cast<unsigned>(wave) ? (whole - wave + WAVES - 1) / WAVES : 0;
+  uint8_t* const mine = lds + wave * kSlots * kSplitSlot;
   const unsigned lds0 = lds_address(mine);
 
   const uint8_t* const abase = a.a.values + m0 * a.a.ld;
@@ -653,7 +601,7 @@ __global__ __launch_bounds__(kSplit * 64, 1) void matmul_split_kernel(MatmulArgs
 
   constexpr int kLoads = 17;
   auto load = [&](unsigned s, unsigned slot, int c) {  // behind the last step it is read once more, for the counts
-    const size_t b = static_cast<size_t>(s < steps ? s : steps - 1) * kSplit + wave;
+    const size_t b = static_cast<size_t>(s < steps ? s : steps - 1) * WAVES + wave;
     const unsigned to = lds0 + slot * kSplitSlot;
     if (c == 0) load_lds4_each(to + 128 * 128, scales + b * scale_step);
     else if (c < 9) load_lds16(to + (c - 1) * 1024, abase + b * kScaleBlock, off_a[c - 1]);
@@ -682,50 +630,22 @@ __global__ __launch_bounds__(kSplit * 64, 1) void matmul_split_kernel(MatmulArgs
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Operands f[2];
-  auto multiply_exactly = [&](const Operands& o) {
+  Operands f[kSlots];
+  auto read = [&](unsigned slot, Operands& o) {
+    read_scales(slot, o);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) read_piece(slot, o, c);
+  };
+  auto far_step = [&](const Operands& o) {
     bool far = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) far = far || far_scale(o.sb >> (8 * i) & 255u) || far_scale(o.sa >> (8 * i) & 255u);
-    const bool near = __builtin_amdgcn_ballot_w64(far) == 0;
-    Wide wb[4];
-    widen_b(o, near ? o.sb : 0x7f7f7f7fu, wb);
-    if (near) multiply_wide(o, wb, acc);
-    else scaled_sums(o, wb, acc, group);
+    return __builtin_amdgcn_ballot_w64(far) != 0;
   };
-
-  if (steps) {
-#pragma unroll
-    for (int c = 0; c < kLoads; ++c) load(0, 0, c);
-#pragma unroll
-    for (int c = 0; c < kLoads; ++c) load(1, 1, c);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
-    read_scales(0, f[0]);
-#pragma unroll
-    for (int c = 0; c < 16; ++c) read_piece(0, f[0], c);
-    auto step = [&](unsigned s, const Operands& now, Operands& then) {
-      const unsigned next = (s + 1) % 2;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // step s is in registers: its slot is free
-#pragma unroll
-      for (int c = 0; c < kLoads; ++c) load(s + 2, s % 2, c);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");  // step s + 1 is in LDS
-      read_scales(next, then);
-      if constexpr (kExact) {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) read_piece(next, then, c);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply_exactly(now);
-      } else {
-        multiply_step(now, acc, [&](int c) { read_piece(next, then, c); });
-      }
-    };
-    for (unsigned s = 0; s < steps; s += 2) {
-      step(s, f[0], f[1]);
-      if (s + 1 < steps) step(s + 1, f[1], f[0]);
-    }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  }
-  if (a.k % kScaleBlock && whole % kSplit == static_cast<unsigned>(wave)) {  // the block cut off by the end of the rows
+  bool far = false;
+  // the block cut off by the end of the rows, zeros behind it
+  const bool cut = a.k % kScaleBlock && whole % WAVES == static_cast<unsigned>(wave);
+  auto load_cut = [&] {
     const size_t k = static_cast<size_t>(whole) * kScaleBlock;
 #pragma unroll 8
     for (int c = 0; c < 16; ++c) {
@@ -736,44 +656,131 @@ __global__ __launch_bounds__(kSplit * 64, 1) void matmul_split_kernel(MatmulArgs
     }
     load_lds4_each(lds0 + 128 * 128, scales + whole * scale_step);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    read_scales(0, f[0]);
+    read(0, f[0]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  if (cut) {
+    load_cut();
+    if constexpr (kExact) {
+      far = far_step(f[0]);
+      Wide wb[4];
+      widen_b(f[0], f[0].sb, wb);
+      multiply_wide(f[0], wb, acc);
+    } else {
+      multiply_step(f[0], acc, [](int) {});
+    }
+  }
+  if (steps && !far) {
 #pragma unroll
-    for (int c = 0; c < 16; ++c) read_piece(0, f[0], c);
-    if constexpr (kExact) multiply_exactly(f[0]);
-    else multiply_step(f[0], acc, [](int) {});
+    for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+      for (int c = 0; c < kLoads; ++c) load(s, s, c);
+    if constexpr (kSlots == 2) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+      read(0, f[0]);
+      auto step = [&](unsigned s, const Operands& now, Operands& then) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // step s is in registers: its slot is free
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) load(s + 2, s % 2, c);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");  // step s + 1 is in LDS
+        read_scales((s + 1) % 2, then);
+        multiply_step(now, acc, [&](int c) { read_piece((s + 1) % 2, then, c); });
+      };
+      for (unsigned s = 0; s < steps; s += 2) {
+        step(s, f[0], f[1]);
+        if (s + 1 < steps) step(s + 1, f[1], f[0]);
+      }
+    } else {
+      for (unsigned s = 0; s < steps; ++s) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        read(0, f[0]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // step s is in registers: its slot is free
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) load(s + 1, 0, c);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kExact) {
+          far = far_step(f[0]);
+          if (far) break;
+          Wide wb[4];
+          widen_b(f[0], f[0].sb, wb);
+          multiply_wide(f[0], wb, acc);
+        } else {
+          multiply_step(f[0], acc, [](int) {});
+        }
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
+  if constexpr (kExact) {
+    if (far) {  // all of this wave's steps again, the slow way
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (unsigned s = 0; s < steps + cut; ++s) {
+        if (s < steps) {
+#pragma unroll
+          for (int c = 0; c < kLoads; ++c) load(s, 0, c);
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          read(0, f[0]);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        } else {
+          load_cut();
+        }
+        Wide wb[4];
+        widen_b(f[0], 0x7f7f7f7fu, wb);
+        scaled_sums(f[0], wb, acc, group);
+      }
+    }
   }
 
+  // The waves' sums, joined: with eight, the upper four hand theirs over first.
+  float* const part = reinterpret_cast<float*>(lds) + wave % 4 * 64 * kSplitPitch;
+  auto hand_over = [&] {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<f32x4*>(part + (4 * j16 + i) * kSplitPitch + 16 * group + 4 * r) =
+            f32x4{acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]};
+  };
   __syncthreads();  // everyone has read its last step
-  float* const part = reinterpret_cast<float*>(lds) + wave * 64 * kSplitPitch;
+  if constexpr (WAVES == 8) {
+    if (wave >= 4) hand_over();
+    __syncthreads();
+    if (wave < 4)
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      *reinterpret_cast<f32x4*>(part + (4 * j16 + i) * kSplitPitch + 16 * group + 4 * r) =
-          f32x4{acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]};
+        for (int r = 0; r < 4; ++r) {
+          const f32x4 more = *reinterpret_cast<const f32x4*>(part + (4 * j16 + i) * kSplitPitch + 16 * group + 4 * r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j][r] += more[j];
+        }
+  }
+  if (wave < 4) hand_over();  // where it read
   __syncthreads();
-  const int row = wave * 16 + lane / 4, col = lane % 4 * 16;  // 16 columns of a row each
+  const int row = threadIdx.x / WAVES, col = threadIdx.x % WAVES * (64 / WAVES);  // 16 or 8 columns of a row each
   if (m0 + row >= a.m) return;
   const float* const sums = reinterpret_cast<const float*>(lds) + row * kSplitPitch + col;
   O* const c = static_cast<O*>(a.c) + (m0 + row) * a.ldc + n0 + col;
   const int left = a.n > n0 + col ? static_cast<int>(std::min<size_t>(a.n - n0 - col, 16)) : 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < kSlots; ++h) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       v[e] = sums[8 * h + e];
 #pragma unroll
-      for (int w = 1; w < kSplit; ++w) v[e] += sums[w * 64 * kSplitPitch + 8 * h + e];
+      for (int w = 1; w < 4; ++w) v[e] += sums[w * 64 * kSplitPitch + 8 * h + e];
     }
     store8(c + 8 * h, left - 8 * h, v);
   }
 }
 
 // The same at 32 x 32, for few rows or few tiles (27 rows of 8192 x 8192: 13.7 us, 4.9 TB/s of weights): 32 rows of A and 32 of B lie in LDS as the 64 rows of a tile would, rows
-// 2 j and 2 j + 1 of A at places 4 j and 4 j + 1, those of B behind them. kSmallSlots steps of a wave are on
-// their way: 128 KB for a CU.
-constexpr int kSmallSlots = 4;
+// 2 j and 2 j + 1 of A at places 4 j and 4 j + 1, those of B behind them. 16 steps of 8 KB are on their
+// way for a CU, shared by its waves.
 constexpr int kSmallSlot = 64 * 128 + 256;
 constexpr int kSmallPitch = 36;  // floats of a row of partial sums
 
@@ -781,18 +788,19 @@ __device__ __forceinline__ void load_lds16_each(unsigned to, const uint8_t* from
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
 
-template <class O, bool kExact>
-__global__ __launch_bounds__(kSplit * 64, 1) void matmul_small_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kSplit * kSmallSlots * kSmallSlot];
-  static_assert(kSplit * 32 * kSmallPitch * 4 <= sizeof(lds), "the partial sums go where the steps were");
+template <class O, bool kExact, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void matmul_small_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
+  constexpr int kSlots = 16 / WAVES;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[WAVES * kSlots * kSmallSlot];
+  static_assert(WAVES * 32 * kSmallPitch * 4 <= sizeof(lds), "the partial sums go where the steps were");
   const int lane = threadIdx.x % 64, group = lane / 16, j16 = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   unsigned tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
   const size_t m0 = static_cast<size_t>(tm) * 32, n0 = static_cast<size_t>(tn) * 32;
   const unsigned whole = static_cast<unsigned>(a.k / kScaleBlock);
-  const unsigned steps = whole > static_cast<unsigned>(wave) ? (whole - wave + kSplit - 1) / kSplit : 0;
-  uint8_t* const mine = lds + wave * kSmallSlots * kSmallSlot;
+  const unsigned steps = whole > static_cast<unsigned>(wave) ? (whole - wave + WAVES - 1) / WAVES : 0;
+  uint8_t* const mine = lds + wave * kSlots * kSmallSlot;
   const unsigned lds0 = lds_address(mine);
 
   // where this lane's part of place 8 c + lane / 8 comes from, from k = 0 on
@@ -814,7 +822,7 @@ __global__ __launch_bounds__(kSplit * 64, 1) void matmul_small_kernel(MatmulArgs
 
   constexpr int kLoads = 9;
   auto load = [&](unsigned s, unsigned slot) {  // behind the last step it is read once more, for the counts
-    const size_t b = static_cast<size_t>(s < steps ? s : steps - 1) * kSplit + wave;
+    const size_t b = static_cast<size_t>(s < steps ? s : steps - 1) * WAVES + wave;
     const unsigned to = lds0 + slot * kSmallSlot;
     load_lds4_each(to + 64 * 128, scales + b * scale_step);
 #pragma unroll
@@ -887,14 +895,14 @@ __global__ __launch_bounds__(kSplit * 64, 1) void matmul_small_kernel(MatmulArgs
   Step f[2];
   if (steps) {
 #pragma unroll
-    for (int s = 0; s < kSmallSlots; ++s) load(s, s);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kSmallSlots - 1) * kLoads) : "memory");
+    for (int s = 0; s < kSlots; ++s) load(s, s);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kSlots - 1) * kLoads) : "memory");
     read(0, f[0]);
     auto step = [&](unsigned s, const Step& now, Step& then) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // step s is in registers: its slot is free
-      load(s + kSmallSlots, s % kSmallSlots);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kSmallSlots - 1) * kLoads) : "memory");  // step s + 1 is in LDS
-      read((s + 1) % kSmallSlots, then);
+      load(s + kSlots, s % kSlots);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kSlots - 1) * kLoads) : "memory");  // step s + 1 is in LDS
+      read((s + 1) % kSlots, then);
       __builtin_amdgcn_sched_barrier(0);
       multiply_all(now);
     };
@@ -904,7 +912,7 @@ __global__ __launch_bounds__(kSplit * 64, 1) void matmul_small_kernel(MatmulArgs
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   }
-  if (a.k % kScaleBlock && whole % kSplit == static_cast<unsigned>(wave)) {  // the block cut off by the end of the rows
+  if (a.k % kScaleBlock && whole % WAVES == static_cast<unsigned>(wave)) {  // the block cut off by the end of the rows
 #pragma unroll
     for (int c = 0; c < 8; ++c)
       *reinterpret_cast<u32x4*>(mine + c * 1024 + lane * 16) = load16(from[c], static_cast<size_t>(whole) * kScaleBlock + piece[c], a.k);
@@ -932,7 +940,7 @@ __global__ __launch_bounds__(kSplit * 64, 1) void matmul_small_kernel(MatmulArgs
   for (int e = 0; e < 8; ++e) {
     v[e] = sums[e];
 #pragma unroll
-    for (int w = 1; w < kSplit; ++w) v[e] += sums[w * 32 * kSmallPitch + e];
+    for (int w = 1; w < WAVES; ++w) v[e] += sums[w * 32 * kSmallPitch + e];
   }
   store8(static_cast<O*>(a.c) + (m0 + row) * a.ldc + n0 + col, a.n > n0 + col ? static_cast<int>(std::min<size_t>(a.n - n0 - col, 8)) : 0, v);
 }
@@ -1169,13 +1177,12 @@ template <class O, bool kExact, int TM, int TN, int kStages> void launch_stage(c
                      0, stream, a, static_cast<unsigned>(tm), static_cast<unsigned>(tn));
 }
 
-template <class O, bool kExact, int MT, int NT, int WAVES, int kAhead> void launch_rows(const MatmulArgs& a, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((a.n + 16 * NT - 1) / (16 * NT)), static_cast<unsigned>((a.m + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((matmul_rows_kernel<O, kExact, MT, NT, WAVES, kAhead>), grid, dim3(WAVES * 64), 0, stream, a);
+template <class O, bool kExact> void launch_rows(const MatmulArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((matmul_rows_kernel<O, kExact>), dim3(static_cast<unsigned>((a.n + 15) / 16)), dim3(kRowWaves * 64), 0, stream, a);
 }
 
 // Which tile makes a product: each kernel has one block on a CU at a time, so it takes ceil(tiles / 256) rounds,
-// each of a start and an end and a time for every 128 k (for every 512 where four waves share k). The
+// each of a start and an end and a time for every 128 k (for every 512 where four waves share k, 1024 for eight). The
 // figures in launch() are microseconds, fitted to these (those in brackets are not chosen). 16-bit:
 //
 //     m x n x k            32 x 32   64 x 64   128 x 128   192 x 128   256 x 128   256 x 256
@@ -1194,15 +1201,16 @@ template <class O, bool kExact, int MT, int NT, int WAVES, int kAhead> void laun
 //     8192 x 1024 x 8192            (132.5)    (104.2)     (109.1)       74.0       (97.4)
 //     4096 x 4096 x 4096                        (110)       (111)        (85)        69.3
 //
-// float32, whose tiles wait for the widening:
+// float32, where eight waves share k: two on a SIMD, one widens while the other multiplies (with four, one
+// to a SIMD: 64 x 64 19.3, 30.2, 36.4 and 78.3 us in rows 1, 2, 4 and 5; 32 x 32 11.4, 16.6 in rows 1 and 2):
 //
 //     m x n x k            32 x 32   64 x 64   256 x 128
-//     64 x 4096 x 4096      11.4     (19.3)                (rows 12.9)
-//     100 x 1024 x 8192     16.6     (30.2)                (rows 21.5)
-//     100 x 8192 x 1024    (19.9)     11.1                 (rows 11.9)
-//     1000 x 1000 x 8000              36.4      (96.9)
-//     1024 x 4096 x 4096             (78.3)      61.2
-//     2048 x 4096 x 4096            (152.5)      79.9
+//     64 x 4096 x 4096       9.5     (13.6)
+//     100 x 1024 x 8192     11.5     (18.9)                (rows of 16 columns 21.5)
+//     100 x 8192 x 1024    (18.3)      9.5                 (rows of 16 columns 11.9)
+//     1000 x 1000 x 8000              24.7      (96.9)
+//     1024 x 4096 x 4096              56.0      (61.2)
+//     2048 x 4096 x 4096             (112)       79.9
 struct Tiles {
   unsigned m, n;
   Tiles(const MatmulArgs& a, size_t tm, size_t tn) : m(static_cast<unsigned>((a.m + tm - 1) / tm)), n(static_cast<unsigned>((a.n + tn - 1) / tn)) {}
@@ -1215,19 +1223,17 @@ struct Tiles {
 
 template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t stream) {
   const Tiles small(a, 32, 32), split(a, 64, 64), mid(a, 128, 128), high(a, 192, 128), tall(a, 256, 128), big(a, 256, 256);
-  const size_t steps = (a.k + kScaleBlock - 1) / kScaleBlock, shared = (steps + kSplit - 1) / kSplit;
-  auto by_small = [&] { hipLaunchKernelGGL((matmul_small_kernel<O, kExact>), small.grid(), dim3(kSplit * 64), 0, stream, a, small.m, small.n); };
-  auto by_split = [&] { hipLaunchKernelGGL((matmul_split_kernel<O, kExact>), split.grid(), dim3(kSplit * 64), 0, stream, a, split.m, split.n); };
+  constexpr int kWaves = kExact ? 8 : 4;  // that share k in the smaller tiles
+  const size_t steps = (a.k + kScaleBlock - 1) / kScaleBlock, shared = (steps + kWaves - 1) / kWaves;
+  auto by_small = [&] { hipLaunchKernelGGL((matmul_small_kernel<O, kExact, kWaves>), small.grid(), dim3(kWaves * 64), 0, stream, a, small.m, small.n); };
+  auto by_split = [&] { hipLaunchKernelGGL((matmul_split_kernel<O, kExact, kWaves>), split.grid(), dim3(kWaves * 64), 0, stream, a, split.m, split.n); };
   // rows too long for the larger tiles' 32-bit offsets
   if (a.a.ld >= (1u << 23) || a.b.ld >= (1u << 23)) return by_small();
   if constexpr (kExact) {
-    // Few rows of A: widened tiles wait for themselves, rows have more waves to take turns (16 x 4096 x 4096
-    // 7.8 us and 10.4; 64 x 8192 x 1024: 7.2 and 10.8, but 64 x 4096 x 4096: 12.9 and 11.4).
-    // 32 columns to a block halve what is read of A, where that leaves a block for most CUs.
-    if (a.m <= 16 && a.n <= 6144) return launch_rows<O, true, 1, 1, 8, 4>(a, stream);
-    if (a.m <= 32) return a.n <= 6144 ? launch_rows<O, true, 2, 1, 8, 1>(a, stream) : launch_rows<O, true, 2, 2, 8, 1>(a, stream);
-    if (a.m <= 64 && a.n > 6144 && a.k <= 2048) return launch_rows<O, true, 4, 2, 8, 1>(a, stream);
-    const double smalls = small.time(3.2, 0.85, shared), splits = split.time(6.0, 1.6, shared), talls = tall.time(5.0, 2.35, steps);
+    // One row of A or a few, for which 16 columns to a block leave fewer CUs without one: 1 x 4096 x 4096 6.3 us
+    // and 8.0 (32 x 32), 16 x 4096 x 4096 7.4 and 8.1, 16 x 8192 x 1024 11.1 and 5.7.
+    if (a.m <= 16 && a.n <= 6144) return launch_rows<O, true>(a, stream);
+    const double smalls = small.time(3.8, 0.95, shared), splits = split.time(6.5, 1.95, shared), talls = tall.time(5.0, 2.35, steps);
     if (smalls <= std::min(splits, talls)) by_small();
     else if (splits <= talls) by_split();
     else launch_stage<O, true, 256, 128, 3>(a, stream);
@@ -1235,7 +1241,7 @@ template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t str
     // One token or so: 16 columns to a block put 1024 < n <= 4096 on twice as many CUs (4096 x 4096: 5.6 us and
     // 6.2; 1024 x 8192: 7.8 both; 1000 x 1024: 5.7 and 5.2; 8192 x 1024: 7.5 and 5.3). From 8 rows on they
     // are no faster.
-    if (a.m <= 4 && a.n > 1024 && a.n <= 4096) return launch_rows<O, false, 1, 1, 8, 4>(a, stream);
+    if (a.m <= 4 && a.n > 1024 && a.n <= 4096) return launch_rows<O, false>(a, stream);
     const double smalls = small.time(2.7, 0.45, shared), splits = split.time(4.5, 0.75, shared), mids = mid.time(5.0, 0.62, steps);
     const double highs = high.time(5.0, 0.88, steps), talls = tall.time(5.0, 1.07, steps);
     const double bigs = a.k >= kScaleBlock ? big.time(6.0, 1.9, steps) : HUGE_VAL;  // it takes at least one whole block
