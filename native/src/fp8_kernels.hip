@@ -242,13 +242,16 @@ __device__ __forceinline__ void store_dx(const NormBackwardArgs& a, size_t row, 
   store_packed<kWhole>(static_cast<T*>(a.dx) + row * a.lddx + col, n, o);
 }
 
+// Threads of a block whose rows take `threads` each: short rows share one, so that a CU makes one partial row.
+constexpr int backward_block(int threads) { return threads <= 64 ? 512 : threads; }
+
 // A block walks rows b, b + G, ...; a thread owns the same columns in all of them and sums its part of
 // dw in registers, so dw costs G partial rows instead of a second pass over dy and h. The next row is
 // requested before the sum over this one is waited for.
 template <class T, class W, int TPR, int NCH, bool kWhole>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_backward_kernel(NormBackwardArgs a) {
-  constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float slot[TPR / 64 * kRows];
+__global__ __launch_bounds__(backward_block(TPR)) void rms_norm_backward_kernel(NormBackwardArgs a) {
+  constexpr int kThreads = backward_block(TPR), kRows = kThreads / TPR;
+  __shared__ float slot[kThreads / 64];
   const int t = threadIdx.x % TPR;
   const size_t step = static_cast<size_t>(gridDim.x) * kRows, row0 = static_cast<size_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
   const int cols = static_cast<int>(a.cols);
@@ -316,7 +319,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_backward_kerne
 #pragma unroll
       for (int j = 0; j < 8; ++j) rows[threadIdx.x / TPR][(c * TPR + t) * 8 + j] = dw[c][j];
     __syncthreads();
-    for (int col = threadIdx.x; col < cols; col += 256) {
+    for (int col = threadIdx.x; col < cols; col += kThreads) {
       float sum = rows[0][col];
 #pragma unroll
       for (int i = 1; i < kRows; ++i) sum += rows[i][col];
@@ -364,40 +367,41 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(NormBackwa
   }
 }
 
-// Sums 64 columns over `rows` rows in 16 interleaved slices, then the slices in order: the same bits on
+// Sums kSumCols columns over `rows` rows in 32 interleaved slices, then the slices in order: the same bits on
 // every run. value(row, col) is what is summed; out(col, sum) takes the result.
+constexpr int kSumCols = 32, kSlices = 1024 / kSumCols;
 template <class F, class O> __device__ __forceinline__ void sum_columns(size_t rows, size_t cols, size_t col0, F value, O out) {
-  __shared__ float slices[16][64];
-  const int lane = threadIdx.x % 64, slice = threadIdx.x / 64;
-  const size_t col = col0 + lane;
+  __shared__ float slices[kSlices][kSumCols];
+  const int at = threadIdx.x % kSumCols, slice = threadIdx.x / kSumCols;
+  const size_t col = col0 + at;
   float s = 0.f;
   if (col < cols) {
 #pragma unroll 8
-    for (size_t r = slice; r < rows; r += 16) s += value(r, col);
+    for (size_t r = slice; r < rows; r += kSlices) s += value(r, col);
   }
-  slices[slice][lane] = s;
+  slices[slice][at] = s;
   __syncthreads();
   if (slice == 0 && col < cols) {
-    s = slices[0][lane];
+    s = slices[0][at];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) s += slices[i][lane];
+    for (int i = 1; i < kSlices; ++i) s += slices[i][at];
     out(col, s);
   }
 }
 
 __global__ __launch_bounds__(1024) void column_sum_kernel(const float* part, size_t rows, size_t cols, float* dw) {
-  sum_columns(rows, cols, static_cast<size_t>(blockIdx.x) * 64, [&](size_t r, size_t c) { return part[r * cols + c]; },
+  sum_columns(rows, cols, static_cast<size_t>(blockIdx.x) * kSumCols, [&](size_t r, size_t c) { return part[r * cols + c]; },
               [&](size_t c, float s) { dw[c] = s; });
 }
 
-// Few rows: one launch. The first blocks make dx, a row each; the others dw, 64 columns each, from dy and
+// Few rows: one launch. The first blocks make dx, a row each; the others dw, kSumCols columns each, from dy and
 // h themselves (they are in the caches).
 template <class T, class W>
 __global__ __launch_bounds__(1024) void rms_norm_backward_few_kernel(NormBackwardArgs a) {
   if (blockIdx.x >= a.rows) {
     const T* const dy = static_cast<const T*>(a.dy);
     const T* const h = static_cast<const T*>(a.h);
-    sum_columns(a.rows, a.cols, (blockIdx.x - a.rows) * 64,
+    sum_columns(a.rows, a.cols, (blockIdx.x - a.rows) * kSumCols,
                 [&](size_t r, size_t c) {
                   return static_cast<float>(dy[r * a.lddy + c]) * (static_cast<float>(h[r * a.ldh + c]) * a.rstd[r]);
                 },
@@ -432,20 +436,23 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_few_kernel(NormBackwar
 constexpr size_t kFewRows = 512, kFewCols = 16384;
 bool few(size_t rows, size_t cols) { return rows <= kFewRows && cols <= kFewCols; }
 
-// Threads of a row, and blocks: enough for the loads of two rows a CU of the widest to be on their way,
-// and few enough for the partial rows to cost little next to dy and h.
-int backward_threads(size_t cols) { return cols <= 1024 ? 64 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024; }
+// Threads of a row.
+int backward_threads(size_t cols) { return cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024; }
+// Blocks: enough for the loads of two rows a CU of the widest to be on their way, and few enough for the
+// weight, the partial rows and their sum to cost little next to dy and h (600 x 8192: 512 blocks 22.6 us,
+// 256 15.8; 16384 x 8192: 177 and 183).
 size_t backward_grid(size_t rows, size_t cols) {
-  const int threads = backward_threads(cols);
-  const size_t blocks = threads == 64 ? (rows + 3) / 4 : rows;
-  return std::min<size_t>(blocks, threads <= 256 ? 1024 : 512);
+  const size_t at_once = static_cast<size_t>(backward_block(backward_threads(cols)) / backward_threads(cols)), sets = (rows + at_once - 1) / at_once;
+  return std::min<size_t>(sets, at_once > 1 ? 512 : std::clamp<size_t>(sets / 32, 256, 512));
 }
 
 template <class T, class W, bool kWhole> void launch_backward_rows(const NormBackwardArgs& a, unsigned grid, hipStream_t stream) {
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(std::max(backward_threads(a.cols), 256)), 0, stream, a);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(backward_block(backward_threads(a.cols))), 0, stream, a);
   };
-  if (a.cols <= 512) go(rms_norm_backward_kernel<T, W, 64, 1, kWhole>);
+  if (a.cols <= 128) go(rms_norm_backward_kernel<T, W, 16, 1, kWhole>);
+  else if (a.cols <= 256) go(rms_norm_backward_kernel<T, W, 32, 1, kWhole>);
+  else if (a.cols <= 512) go(rms_norm_backward_kernel<T, W, 64, 1, kWhole>);
   else if (a.cols <= 1024) go(rms_norm_backward_kernel<T, W, 64, 2, kWhole>);
   else if (a.cols <= 2048) go(rms_norm_backward_kernel<T, W, 256, 1, kWhole>);
   else if (a.cols <= 4096) go(rms_norm_backward_kernel<T, W, 512, 1, kWhole>);
@@ -455,7 +462,7 @@ template <class T, class W, bool kWhole> void launch_backward_rows(const NormBac
 }
 
 template <class T, class W> void launch_backward(const NormBackwardArgs& a, hipStream_t stream) {
-  const size_t sums = (a.cols + 63) / 64;
+  const size_t sums = (a.cols + kSumCols - 1) / kSumCols;
   if (few(a.rows, a.cols)) {
     hipLaunchKernelGGL((rms_norm_backward_few_kernel<T, W>), dim3(static_cast<unsigned>(a.rows + sums)), dim3(1024), 0, stream, a);
   } else {
@@ -483,7 +490,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeArgs a) {
     const size_t row = items >> 32 ? item / blocks : static_cast<unsigned>(item) / blocks;
     const size_t block = item - row * blocks, col = block * kScaleBlock + c;
     const int n = item < items && a.cols > col ? static_cast<int>(std::min<size_t>(a.cols - col, 8)) : 0;
-    const Packed8<T> v = load_packed<kWhole>(static_cast<const T*>(a.x) + row * a.ldx + col, n);
+    const Packed8<T> v = load_packed<kWhole, T, false>(static_cast<const T*>(a.x) + row * a.ldx + col, n);
     const unsigned byte = scale_byte(max16(largest_of(magnitudes(v))));
     store_bytes<kWhole>(a.rows_out.values + row * a.rows_out.ld + col, n, u32x2{pack_four(v, 0, byte), pack_four(v, 1, byte)});
     if (n > 0 && c == 0) a.rows_out.scales[block * a.rows_out.ld_scales + row] = static_cast<uint8_t>(byte);
@@ -525,7 +532,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs a) {
     const T* const x = static_cast<const T*>(a.x) + (r0 + r) * a.ldx + c0 + c;
     Packed8<T> v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = load_packed<kWhole>(x + i * a.ldx, i < m ? n : 0);
+    for (int i = 0; i < 8; ++i) v[i] = load_packed<kWhole, T, false>(x + i * a.ldx, i < m ? n : 0);
     if (a.rows_out.values) {
       unsigned bytes[8];
 #pragma unroll
