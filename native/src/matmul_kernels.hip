@@ -1270,8 +1270,8 @@ void fp8_matmul(const MatmulArgs& a, LayerType out, hipStream_t stream) {
   check(reinterpret_cast<uintptr_t>(a.a.scales) % 4 == 0 && a.a.ld_scales % 4 == 0 &&
             reinterpret_cast<uintptr_t>(a.b.scales) % 4 == 0 && a.b.ld_scales % 4 == 0,
         "fp8: the scales of a block must start on a 4-byte boundary");
-  check(a.m <= (1u << 20) && a.n <= (1u << 24) && (a.m + 63) / 64 * ((a.n + 63) / 64) <= (size_t(1) << 24),
-        "fp8_matmul: at most 2^20 rows and 2^24 columns of C, and 2^36 values");
+  check(a.m <= (size_t(1) << 32) && a.n <= (size_t(1) << 32) && (a.m + 63) / 64 * ((a.n + 63) / 64) <= (size_t(1) << 24),
+        "fp8_matmul: at most 2^32 rows and columns of C, and 2^36 values");
   switch (out) {
     case LayerType::kF32: launch<float, true>(a, stream); break;
     case LayerType::kBF16: launch<__bf16, false>(a, stream); break;

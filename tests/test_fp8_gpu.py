@@ -548,3 +548,51 @@ def test_two_streams_at_once(fp8):
         for run in got[k]:
             for key in run:
                 assert torch.equal(run[key], want[k][key]), (k, key)
+
+
+def test_more_values_than_32_bits_count(fp8):
+    """2.3e9 values: the last rows come out as they do by themselves."""
+    rows, cols, tail = 70000, 32768, 112  # 70000 = 546 * 128 + 112
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x.view(torch.int16).copy_(torch.arange(cols, dtype=torch.int16, device="cuda") % 199 + 16100)
+    x[-tail:].mul_(torch.randn(tail, 1, device="cuda").bfloat16()).add_(torch.randn(tail, cols, device="cuda").bfloat16())
+    end = x[-tail:].clone()
+    for layout in ("rows", "both", "tiles"):
+        whole, part = fp8.quantize(x, layout=layout), fp8.quantize(end, layout=layout)
+        if layout == "both":
+            assert torch.equal(bits_of(whole[1].values[:, -tail:]), bits_of(part[1].values))
+            assert torch.equal(bits_of(whole[1].scales[:, -1]), bits_of(part[1].scales[:, -1]))
+            whole, part = whole[0], part[0]
+        assert torch.equal(bits_of(whole.values[-tail:]), bits_of(part.values)), layout
+        n = 1 if layout == "tiles" else tail
+        assert torch.equal(bits_of(whole.scales[-n:]), bits_of(part.scales[-n:])), layout
+        del whole, part
+    w = torch.randn(cols, device="cuda").bfloat16()
+    whole, part = fp8.rms_norm(x, w, normed=True), fp8.rms_norm(end, w, normed=True)
+    assert torch.equal(bits_of(whole.values[-tail:]), bits_of(part.values)) and torch.equal(whole.y[-tail:], part.y)
+    assert torch.equal(bits_of(whole.scales[-tail:]), bits_of(part.scales)) and torch.equal(whole.rstd[-tail:], part.rstd)
+    rstd = whole.rstd
+    del whole
+    dx, dw = fp8.rms_norm_backward(x, x, w, rstd)
+    dx1, _ = fp8.rms_norm_backward(end, end, w, part.rstd)
+    assert torch.equal(dx[-tail:], dx1)
+    want = sum((x[i:i + 5000].double().square() * rstd[i:i + 5000, None].double()).sum(0) for i in range(0, rows, 5000))
+    assert ((dw.double() - want).abs() <= (rows + 8) * U * want).all()
+
+
+def bits_of(t):
+    return t.contiguous().view(torch.uint8)
+
+
+@pytest.mark.parametrize("m,n", [((1 << 21) + 5, 2100), (70, (1 << 24) + 9)])
+def test_products_of_more_values_than_32_bits_count(fp8, m, n):
+    k = 130
+    def rows_of(seed, rows):
+        small, small64 = operand(fp8, seed, 512, k)
+        i = torch.arange(rows, device="cuda") % 509
+        return fp8.Quantized(torch.nn.functional.pad(bits_of(small.values), (0, 14))[i].view(torch.float8_e4m3fn)[:, :k],
+                             bits_of(small.scales).t()[:, i].contiguous().view(torch.float8_e8m0fnu).t()), small64
+    (a, a64), (b, b64) = rows_of(1, m), rows_of(2, n)
+    c = fp8.matmul(a, b)
+    for r, q in ((slice(0, 70), slice(0, 300)), (slice(m - 70, m), slice(n - 300, n)), (slice(m // 2, m // 2 + 64), slice(n // 2, n // 2 + 99))):
+        check_product(c[r, q], a64[np.arange(m)[r] % 509], b64[np.arange(n)[q] % 509], k)
