@@ -596,3 +596,18 @@ def test_products_of_more_values_than_32_bits_count(fp8, m, n):
     c = fp8.matmul(a, b)
     for r, q in ((slice(0, 70), slice(0, 300)), (slice(m - 70, m), slice(n - 300, n)), (slice(m // 2, m // 2 + 64), slice(n // 2, n // 2 + 99))):
         check_product(c[r, q], a64[np.arange(m)[r] % 509], b64[np.arange(n)[q] % 509], k)
+
+
+@pytest.mark.parametrize("cols", [200, 4096, 40000])
+def test_what_a_call_returns_does_not_overlap(fp8, cols):
+    """Small results share an allocation: writing to one leaves the others."""
+    x, w = torch.randn(3, cols, device="cuda"), torch.randn(cols, device="cuda")
+    n = fp8.rms_norm(x, w, residual=x, normed=True)
+    results = {"norm": [n.h, n.values, n.scales, n.y, n.rstd], "both": [t for q in fp8.quantize(x, layout="both") for t in q],
+               "tiles": list(fp8.quantize(x, layout="tiles")), "backward": list(fp8.rms_norm_backward(x, n.h, w, n.rstd))}
+    for name, got in results.items():
+        want = [bits_of(t).clone() for t in got]
+        for i, t in enumerate(got):
+            (t if t.dtype == torch.float32 else t.view(torch.uint8)).fill_(85)
+            for j, u in enumerate(got):
+                assert j <= i or torch.equal(bits_of(u), want[j]), (name, i, j)
