@@ -145,10 +145,11 @@ template <class T> __device__ __forceinline__ void keep_packed(Packed8<T>& p) {
 template <bool kWhole> __device__ __forceinline__ void store_bytes(uint8_t* p, int n, u32x2 v) {
   if (kWhole ? n > 0 : n >= 8) {
     __builtin_nontemporal_store(v, reinterpret_cast<u32x2*>(p));
-  } else if (!kWhole) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = static_cast<uint8_t>((j < 4 ? v.x : v.y) >> (8 * (j & 3)));
+  } else if (!kWhole && n > 0) {  // in parts of 4, 2 and 1, on boundaries of their sizes
+    const unsigned rest = n & 4 ? v.y : v.x;
+    if (n & 4) *reinterpret_cast<unsigned*>(p) = v.x;
+    if (n & 2) *reinterpret_cast<unsigned short*>(p + (n & 4)) = static_cast<unsigned short>(rest);
+    if (n & 1) p[n & 6] = static_cast<uint8_t>(rest >> (n & 2 ? 16 : 0));
   }
 }
 
