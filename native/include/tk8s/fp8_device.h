@@ -166,15 +166,16 @@ template <class T> __device__ __forceinline__ void load8(const T* p, int n, floa
 }
 
 // p[0..n-1] = v[0..n-1], one rounding to T.
-template <class T> __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
-  if (n >= 8) {
-    Eight<T> e;
+template <class T, int N> __device__ __forceinline__ void store_some(T* p, int n, const float (&v)[N]) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Some { T v[N]; };
+  if (n >= N) {
+    Some e;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e.v[j] = static_cast<T>(v[j]);
-    *reinterpret_cast<Eight<T>*>(p) = e;
+    for (int j = 0; j < N; ++j) e.v[j] = static_cast<T>(v[j]);
+    *reinterpret_cast<Some*>(p) = e;
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < N; ++j)
       if (j < n) p[j] = static_cast<T>(v[j]);
   }
 }

@@ -331,7 +331,7 @@ __global__ __launch_bounds__(backward_block(TPR)) void rms_norm_backward_kernel(
     return;
   }
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) store8(part + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, dw[c]);
+  for (int c = 0; c < NCH; ++c) store_some(part + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, dw[c]);
 }
 
 // Rows longer than the registers of a block hold: dy and h are read again for dx, and the partial sums
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(NormBackwa
         dw[j] = fmaf(unpack(dy, j), xh, dw[j]);
         inner = fmaf(unpack(dy, j) * unpack(w, j), xh, inner);
       }
-      store8(part + col, cols - col, dw);
+      store_some(part + col, cols - col, dw);
     }
     const float mean = row_sum<1024>(inner, slot) / cols;
     for (int col = threadIdx.x * 8; col < cols; col += 8192) {

@@ -238,6 +238,43 @@ template <int kLeft> __device__ __forceinline__ void wait_and_meet() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// Lanes change values: the upper 32 of x with the lower 32 of y; odd 16 of x with the even 16 of y behind which they lie.
+__device__ __forceinline__ void swap32(float& x, float& y) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  x = __uint_as_float(r[0]);
+  y = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void swap16(float& x, float& y) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  x = __uint_as_float(r[0]);
+  y = __uint_as_float(r[1]);
+}
+
+// 64 columns of C from c on, of `left` there are: a lane has 16 neighbouring ones of its row, 16 group + 4 r + j
+// in sums[j][r]. They change lanes first, so that the four lanes of a row write 64 neighbouring bytes with
+// every store instead of 16 here and there (8192 x 8192 x 1024, 16-bit: 117 -> 104 us; 2048 x 4096 x 4096,
+// 32-bit: 84 -> 75).
+template <class O> __device__ __forceinline__ void store_row(O* c, bool inside, int left, const f32x4 (&sums)[4], int group) {
+  constexpr int kPer = 16 / sizeof(O), kStores = 16 / kPer;
+  float v[kStores][kPer];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e / kPer][e % kPer] = sums[e % 4][e / 4];
+#pragma unroll
+  for (int s = 0; s < kStores / 2; ++s)
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) swap32(v[s][e], v[s + kStores / 2][e]);
+  if constexpr (kStores == 4) {
+#pragma unroll
+    for (int s = 0; s < 4; s += 2)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) swap16(v[s][e], v[s + 1][e]);
+  }
+  if (!inside) return;
+  const int at = kPer * (kStores == 4 ? group : group % 2 * 2 + group / 2);
+#pragma unroll
+  for (int s = 0; s < kStores; ++s) store_some(c + 4 * kPer * s + at, left - 4 * kPer * s - at, v[s]);
+}
+
 // What a wave multiplies in one step: four tiles of 16 rows of each operand and their scales.
 struct Operands {
   Fragment b[4], a[4];
@@ -318,8 +355,8 @@ __device__ __forceinline__ void scaled_sums(const Operands& f, const Wide (&wb)[
 // of the step kStages ahead are requested (straight into LDS, no registers). One barrier a step
 // says both that the next step has arrived and that the slot to be refilled has been read. What
 // bounds it is the time a request takes against kStages - 1 steps: LDS is as full of bytes on
-// their way as it can be. 1024 x 4096 x 4096, 16-bit: 24.6 us, 1400 TFLOP/s (128 x 128); 2048 rows: 39.4, 1740
-// (256 x 128). 32-bit sums, 4096 x 4096 x 10007: 296 us, 1130 TFLOP/s, the matrix units busy half of the
+// their way as it can be. 1024 x 4096 x 4096, 16-bit: 24.2 us, 1420 TFLOP/s (128 x 128); 2048 rows: 39.2, 1750
+// (256 x 128). 32-bit sums, 4096 x 4096 x 10007: 281 us, 1200 TFLOP/s, the matrix units busy half of the
 // time and the vector units with the widening.
 template <class O, bool kExact, int TM, int TN, int kStages>
 __global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
@@ -425,20 +462,12 @@ __global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(
 
   auto store = [&](const f32x4 (&sums)[4][4]) {
     // lane: row 4 * j16 + i, columns 16 * group + 4 r + j
-    const size_t mw = m0 + wm * 64, col = n0 + wn * 64 + 16 * group;
-    const int left = col < a.n ? static_cast<int>(std::min<size_t>(a.n - col, 16)) : 0;
+    const size_t mw = m0 + wm * 64, col = n0 + wn * 64;
+    const int left = col < a.n ? static_cast<int>(std::min<size_t>(a.n - col, 64)) : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const size_t row = mw + 4 * j16 + i;
-      if (row >= a.m) continue;
-      O* const c = static_cast<O*>(a.c) + row * a.ldc + col;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = sums[i][e % 4][2 * h + e / 4];
-        store8(c + 8 * h, left - 8 * h, v);
-      }
+      store_row(static_cast<O*>(a.c) + row * a.ldc + col, row < a.m, left, sums[i], group);
     }
   };
 
@@ -554,7 +583,7 @@ __global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(
 // ------------------------------------------------------------------------------------------
 // Small tiles, shared along k
 // ------------------------------------------------------------------------------------------
-// Where larger tiles would leave most of the chip idle (100 x 8192 x 8192: 17.3 us, 128 x 128 31.5): a block makes
+// Where larger tiles would leave most of the chip idle (100 x 8192 x 8192: 17.4 us, 128 x 128 31.8): a block makes
 // 64 x 64 of C, and each of its WAVES waves takes every WAVES-th step of 128 k for itself -- its own slots in LDS,
 // eight in all, waited for by count, no barrier -- with the sums joined in LDS at the end, in
 // order. Four waves keep two steps each on their way; eight (32-bit results) one, and two to a SIMD.
@@ -762,21 +791,21 @@ __global__ __launch_bounds__(WAVES * 64) void matmul_split_kernel(MatmulArgs a, 
   }
   if (wave < 4) hand_over();  // where it read
   __syncthreads();
-  const int row = threadIdx.x / WAVES, col = threadIdx.x % WAVES * (64 / WAVES);  // 16 or 8 columns of a row each
-  if (m0 + row >= a.m) return;
-  const float* const sums = reinterpret_cast<const float*>(lds) + row * kSplitPitch + col;
-  O* const c = static_cast<O*>(a.c) + (m0 + row) * a.ldc + n0 + col;
-  const int left = a.n > n0 + col ? static_cast<int>(std::min<size_t>(a.n - n0 - col, 16)) : 0;
+  constexpr int kPer = 16 / sizeof(O), kRows = WAVES * kPer;  // columns of a thread, rows that all of them store at once
+  const int col = threadIdx.x % (64 / kPer) * kPer;
+  const int left = a.n > n0 + col ? static_cast<int>(std::min<size_t>(a.n - n0 - col, kPer)) : 0;
 #pragma unroll
-  for (int h = 0; h < kSlots; ++h) {
-    float v[8];
+  for (int row = threadIdx.x / (64 / kPer); row < 64; row += kRows) {
+    if (m0 + row >= a.m) return;
+    const float* const sums = reinterpret_cast<const float*>(lds) + row * kSplitPitch + col;
+    float v[kPer];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = sums[8 * h + e];
+    for (int e = 0; e < kPer; ++e) {
+      v[e] = sums[e];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) v[e] += sums[w * 64 * kSplitPitch + 8 * h + e];
+      for (int w = 1; w < 4; ++w) v[e] += sums[w * 64 * kSplitPitch + e];
     }
-    store8(c + 8 * h, left - 8 * h, v);
+    store_some(static_cast<O*>(a.c) + (m0 + row) * a.ldc + n0 + col, left, v);
   }
 }
 
@@ -933,18 +962,18 @@ __global__ __launch_bounds__(WAVES * 64) void matmul_small_kernel(MatmulArgs a, 
       *reinterpret_cast<f32x4*>(part + (2 * j16 + i) * kSmallPitch + 8 * group + 4 * h) =
           f32x4{acc[i][0][2 * h], acc[i][1][2 * h], acc[i][0][2 * h + 1], acc[i][1][2 * h + 1]};
   __syncthreads();
-  if (wave >= 2) return;
-  const int row = threadIdx.x / 4, col = threadIdx.x % 4 * 8;
-  if (m0 + row >= a.m) return;
+  constexpr int kPer = 16 / sizeof(O);  // columns of a thread
+  const int row = threadIdx.x / (32 / kPer), col = threadIdx.x % (32 / kPer) * kPer;
+  if (row >= 32 || m0 + row >= a.m) return;
   const float* const sums = reinterpret_cast<const float*>(lds) + row * kSmallPitch + col;
-  float v[8];
+  float v[kPer];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < kPer; ++e) {
     v[e] = sums[e];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) v[e] += sums[w * 32 * kSmallPitch + e];
   }
-  store8(static_cast<O*>(a.c) + (m0 + row) * a.ldc + n0 + col, a.n > n0 + col ? static_cast<int>(std::min<size_t>(a.n - n0 - col, 8)) : 0, v);
+  store_some(static_cast<O*>(a.c) + (m0 + row) * a.ldc + n0 + col, a.n > n0 + col ? static_cast<int>(std::min<size_t>(a.n - n0 - col, kPer)) : 0, v);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -960,7 +989,7 @@ __global__ __launch_bounds__(WAVES * 64) void matmul_small_kernel(MatmulArgs a, 
 // about four phases to arrive. Every wave issues the same nine loads a step between its matrix
 // instructions (256 bytes of scales, four pieces of 1 KiB of B, two of A's first half; two of A's
 // second half), which makes the counts the same for all.
-// 8192 x 8192 x 8192: 444 us, 2480 TFLOP/s at the 2.0 GHz that power leaves; no access to LDS conflicts.
+// 8192 x 8192 x 8192: 428 us, 2570 TFLOP/s at the 2.0 GHz that power leaves; no access to LDS conflicts.
 // LDS: two slots each of B's 256 rows, of A's first and of its second halves (128 rows each) and of the
 // scales, so that both slots lie within the reach of one address.
 constexpr int kBigB = 0, kBigA = 2 * 256 * 128, kBigHalf = 128 * 128, kBigScales = 2 * 512 * 128;
@@ -1151,22 +1180,14 @@ __global__ __launch_bounds__(512, 2) void matmul_big_kernel(MatmulArgs a, unsign
   if (whole % 2) step(whole - 1, kHalf0);
   if (wm == 0) phase_end();
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may still be on its way to LDS when the block ends
-  const size_t mw = m0 + wm * 128, col = n0 + wn * 64 + 16 * group;
-  const int left = col < a.n ? static_cast<int>(std::min<size_t>(a.n - col, 16)) : 0;
+  const size_t mw = m0 + wm * 128, col = n0 + wn * 64;
+  const int left = col < a.n ? static_cast<int>(std::min<size_t>(a.n - col, 64)) : 0;
 #pragma unroll
   for (int g = 0; g < 2; ++g)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const size_t row = mw + 64 * g + 4 * j16 + i;
-      if (row >= a.m) continue;
-      O* const c = static_cast<O*>(a.c) + row * a.ldc + col;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = acc[g * 4 + i][e % 4][2 * h + e / 4];
-        store8(c + 8 * h, left - 8 * h, v);
-      }
+      store_row(static_cast<O*>(a.c) + row * a.ldc + col, row < a.m, left, acc[g * 4 + i], group);
     }
 }
 
@@ -1195,25 +1216,32 @@ template <class O, bool kExact> void launch_rows(const MatmulArgs& a, hipStream_
 //     500 x 500 x 8000      10.3     (17.9)     (33.1)
 //     27 x 14336 x 4096    (14.9)     13.5                                                    (rows 23.4)
 //     100 x 8192 x 8192    (33.1)     17.3      (31.5)
-//     256 x 4096 x 4096    (23.4)     12.1      (19.8)      (27.3)      (29.8)      (50.7)
-//     512 x 4096 x 4096               20.4      (21.0)      (28.6)      (31.3)      (51.3)
-//     2000 x 2000 x 2000             (31.5)      21.3       (24.5)      (26.1)      (36.7)
-//     1024 x 4096 x 4096             (38.4)      24.6       (31.6)      (33.4)      (53.3)
-//     777 x 5003 x 4432              (57.6)     (47.6)       36.1       (39.5)      (58.1)
-//     2048 x 4096 x 4096             (74.0)     (50.5)      (58.7)       39.4       (57.2)
-//     8192 x 1024 x 8192            (132.5)    (104.2)     (109.1)       74.0       (97.4)
-//     4096 x 4096 x 4096                        (110)       (111)        (85)        69.3
+//     256 x 4096 x 4096    (23.7)     12.8      (20.1)      (27.3)      (29.6)      (50.7)
+//     512 x 4096 x 4096               21.4      (21.3)      (28.6)      (31.4)      (51.6)
+//     2000 x 2000 x 2000             (34.1)      20.3       (23.7)      (26.6)      (36.6)
+//     1024 x 4096 x 4096             (41.0)      24.2       (31.3)      (33.9)      (52.8)
+//     607 x 12416 x 256              (33.4)      16.6       (21.3)      (21.5)      (20.1)
+//     777 x 5003 x 4432              (56.5)     (47.9)       34.9       (38.6)      (58.2)
+//     2521 x 2176 x 128              (24.5)     (15.0)       12.1       (13.4)      (18.0)
+//     2048 x 4096 x 4096             (78.8)     (46.9)      (58.8)       39.2       (56.4)
+//     8192 x 1024 x 8192             (130.9)    (91.8)      (98.2)       68.3       (96.4)
+//     3000 x 8192 x 2048             (156.4)    (86.5)      (79.3)       70.8       (71.3)
+//     4096 x 4096 x 512              (76.8)     (32.9)      (33.5)      (29.3)       23.2
+//     4096 x 4096 x 4096             (150.5)   (100.7)      (93.9)      (76.1)       65.1
+//     8192 x 8192 x 1024             (316.4)   (149.3)     (141.6)     (123.4)       98.0
 //
 // float32, where eight waves share k: two on a SIMD, one widens while the other multiplies (with four, one
 // to a SIMD: 64 x 64 19.3, 30.2, 36.4 and 78.3 us in rows 1, 2, 4 and 5; 32 x 32 11.4, 16.6 in rows 1 and 2):
 //
 //     m x n x k            32 x 32   64 x 64   256 x 128
-//     64 x 4096 x 4096       9.5     (13.6)
-//     100 x 1024 x 8192     11.5     (18.9)                (rows of 16 columns 21.5)
-//     100 x 8192 x 1024    (18.3)      9.5                 (rows of 16 columns 11.9)
-//     1000 x 1000 x 8000              24.7      (96.9)
-//     1024 x 4096 x 4096              56.0      (61.2)
-//     2048 x 4096 x 4096             (112)       79.9
+//     64 x 4096 x 4096       9.7     (13.7)     (50.2)
+//     100 x 1024 x 8192     11.6     (19.3)     (93.0)     (rows of 16 columns 21.5)
+//     100 x 8192 x 1024    (18.8)      9.8      (19.3)     (rows of 16 columns 11.9)
+//     1000 x 1000 x 8000   (49.6)     24.9     (101.2)
+//     1024 x 4096 x 4096  (113.5)     58.3      (61.6)
+//     2394 x 1408 x 2048   (70.2)    (40.9)      38.1
+//     2521 x 2176 x 128    (62.6)    (36.4)      16.5
+//     2048 x 4096 x 4096            (112.8)      70.6
 struct Tiles {
   unsigned m, n;
   Tiles(const MatmulArgs& a, size_t tm, size_t tn) : m(static_cast<unsigned>((a.m + tm - 1) / tm)), n(static_cast<unsigned>((a.n + tn - 1) / tn)) {}
@@ -1236,7 +1264,7 @@ template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t str
     // One row of A or a few, for which 16 columns to a block leave fewer CUs without one: 1 x 4096 x 4096 6.3 us
     // and 8.0 (32 x 32), 16 x 4096 x 4096 7.4 and 8.1, 16 x 8192 x 1024 11.1 and 5.7.
     if (a.m <= 16 && a.n <= 6144) return launch_rows<O, true>(a, stream);
-    const double smalls = small.time(3.8, 0.95, shared), splits = split.time(6.5, 1.95, shared), talls = tall.time(5.0, 2.35, steps);
+    const double smalls = small.time(3.8, 0.95, shared), splits = split.time(6.5, 1.95, shared), talls = tall.time(10.0, 1.75, steps);
     if (smalls <= std::min(splits, talls)) by_small();
     else if (splits <= talls) by_split();
     else launch_stage<O, true, 256, 128, 3>(a, stream);
@@ -1245,9 +1273,9 @@ template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t str
     // 6.2; 1024 x 8192: 7.8 both; 1000 x 1024: 5.7 and 5.2; 8192 x 1024: 7.5 and 5.3). From 8 rows on they
     // are no faster.
     if (a.m <= 4 && a.n > 1024 && a.n <= 4096) return launch_rows<O, false>(a, stream);
-    const double smalls = small.time(2.7, 0.45, shared), splits = split.time(4.5, 0.75, shared), mids = mid.time(5.0, 0.62, steps);
-    const double highs = high.time(5.0, 0.88, steps), talls = tall.time(5.0, 1.07, steps);
-    const double bigs = a.k >= kScaleBlock ? big.time(6.0, 1.9, steps) : HUGE_VAL;  // it takes at least one whole block
+    const double smalls = small.time(2.7, 0.45, shared), splits = split.time(4.5, 0.75, shared), mids = mid.time(6.0, 0.55, steps);
+    const double highs = high.time(8.5, 0.78, steps), talls = tall.time(10.0, 0.95, steps);
+    const double bigs = a.k >= kScaleBlock ? big.time(13.0, 1.6, steps) : HUGE_VAL;  // it takes at least one whole block
     const double least = std::min({smalls, splits, mids, highs, talls, bigs});
     if (least == smalls) by_small();
     else if (least == splits) by_split();
