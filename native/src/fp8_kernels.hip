@@ -440,13 +440,18 @@ constexpr size_t kFewRows = 512, kFewCols = 16384;
 bool few(size_t rows, size_t cols) { return rows <= kFewRows && cols <= kFewCols; }
 
 // Threads of a row.
-int backward_threads(size_t cols) { return cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 256 : cols <= 4096 ? 512 : 1024; }
-// Blocks: enough for the loads of two rows a CU of the widest to be on their way, and few enough for the
-// weight, the partial rows and their sum to cost little next to dy and h (600 x 8192: 512 blocks 22.6 us,
-// 256 15.8; 16384 x 8192: 177 and 183).
+int backward_threads(size_t cols) { return cols <= 128 ? 16 : cols <= 256 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 256 : cols <= 2560 ? 320 : cols <= 4096 ? 512 : 1024; }
+// Blocks: enough for the loads of two rows a CU of the widest to be on their way, of narrower ones more, and few
+// enough for the weight, the partial rows and their sum to cost little next to dy and h (600 x 8192: 512 blocks
+// 22.6 us, 256 15.8; 16384 x 8192: 177 and 183; 11638 x 4096, 32-bit: 727 blocks 154, 640 165, 364 180; 20000 x
+// 2048, 16-bit: 512 blocks 59, 640 65; 5000 x 5000: 312 blocks 58, 256 43).
 size_t backward_grid(size_t rows, size_t cols) {
-  const size_t at_once = static_cast<size_t>(backward_block(backward_threads(cols)) / backward_threads(cols)), sets = (rows + at_once - 1) / at_once;
-  return std::min<size_t>(sets, at_once > 1 ? 512 : std::clamp<size_t>(sets / 32, 256, 512));
+  const int threads = backward_threads(cols);
+  const size_t at_once = static_cast<size_t>(backward_block(threads) / threads), sets = (rows + at_once - 1) / at_once;
+  const size_t most = at_once > 1   ? 512
+                      : cols > 4096 ? (sets / 32 >= 512 ? 512 : 256)
+                                    : std::clamp<size_t>(sets / 16, 256, threads > 256 ? 768 : 512);
+  return std::min(sets, most);
 }
 
 template <class T, class W, bool kWhole> void launch_backward_rows(const NormBackwardArgs& a, unsigned grid, hipStream_t stream) {
@@ -458,6 +463,7 @@ template <class T, class W, bool kWhole> void launch_backward_rows(const NormBac
   else if (a.cols <= 512) go(rms_norm_backward_kernel<T, W, 64, 1, kWhole>);
   else if (a.cols <= 1024) go(rms_norm_backward_kernel<T, W, 64, 2, kWhole>);
   else if (a.cols <= 2048) go(rms_norm_backward_kernel<T, W, 256, 1, kWhole>);
+  else if (a.cols <= 2560) go(rms_norm_backward_kernel<T, W, 320, 1, kWhole>);
   else if (a.cols <= 4096) go(rms_norm_backward_kernel<T, W, 512, 1, kWhole>);
   else if (a.cols <= 8192) go(rms_norm_backward_kernel<T, W, 1024, 1, kWhole>);
   else if (a.cols <= 16384) go(rms_norm_backward_kernel<T, W, 1024, 2, kWhole>);

@@ -356,7 +356,7 @@ __device__ __forceinline__ void scaled_sums(const Operands& f, const Wide (&wb)[
 // says both that the next step has arrived and that the slot to be refilled has been read. What
 // bounds it is the time a request takes against kStages - 1 steps: LDS is as full of bytes on
 // their way as it can be. 1024 x 4096 x 4096, 16-bit: 24.2 us, 1420 TFLOP/s (128 x 128); 2048 rows: 39.2, 1750
-// (256 x 128). 32-bit sums, 4096 x 4096 x 10007: 281 us, 1200 TFLOP/s, the matrix units busy half of the
+// (256 x 128). 32-bit sums, 4096 x 4096 x 10007: 281 - 301 us, 1120 - 1200 TFLOP/s, the matrix units busy half of the
 // time and the vector units with the widening.
 template <class O, bool kExact, int TM, int TN, int kStages>
 __global__ __launch_bounds__(TM / 64 * (TN / 64) * 64) void matmul_stage_kernel(MatmulArgs a, unsigned tiles_m, unsigned tiles_n) {
@@ -989,7 +989,7 @@ __global__ __launch_bounds__(WAVES * 64) void matmul_small_kernel(MatmulArgs a, 
 // about four phases to arrive. Every wave issues the same nine loads a step between its matrix
 // instructions (256 bytes of scales, four pieces of 1 KiB of B, two of A's first half; two of A's
 // second half), which makes the counts the same for all.
-// 8192 x 8192 x 8192: 428 us, 2570 TFLOP/s at the 2.0 GHz that power leaves; no access to LDS conflicts.
+// 8192 x 8192 x 8192: 428 - 452 us, 2430 - 2570 TFLOP/s at the 2.0 GHz that power leaves; no access to LDS conflicts.
 // LDS: two slots each of B's 256 rows, of A's first and of its second halves (128 rows each) and of the
 // scales, so that both slots lie within the reach of one address.
 constexpr int kBigB = 0, kBigA = 2 * 256 * 128, kBigHalf = 128 * 128, kBigScales = 2 * 512 * 128;

@@ -246,7 +246,7 @@ def test_norm_of_nothing(fp8):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("more", [False, True])
-@pytest.mark.parametrize("rows,cols", NORM_SHAPES + [(1500, 260), (1025, 17), (2500, 126), (700, 250), (1100, 1003), (600, 437), (1026, 2047), (515, 4098), (9000, 129)])
+@pytest.mark.parametrize("rows,cols", NORM_SHAPES + [(1500, 260), (1025, 17), (2500, 126), (700, 250), (1100, 1003), (600, 437), (1026, 2047), (515, 4098), (9000, 129), (9000, 2404), (17000, 2100)])
 def test_norm_backward_matches_the_oracle(fp8, dtype, more, rows, cols):
     h = randn(rows + cols, rows, cols, dtype=dtype, spread=2.0)
     dy = randn(8, rows, cols, dtype=dtype)
