@@ -1246,7 +1246,10 @@ struct Tiles {
   unsigned m, n;
   Tiles(const MatmulArgs& a, size_t tm, size_t tn) : m(static_cast<unsigned>((a.m + tm - 1) / tm)), n(static_cast<unsigned>((a.n + tn - 1) / tn)) {}
   dim3 grid() const { return dim3(m * n); }
-  double time(double ends, double step, size_t steps) const {
+  // a launch has fewer than 2^32 threads
+  bool fit(size_t threads) const { return static_cast<size_t>(m) * n * threads >> 32 == 0; }
+  double time(size_t threads, double ends, double step, size_t steps) const {
+    if (!fit(threads)) return HUGE_VAL;
     const size_t rounds = (static_cast<size_t>(m) * n + 255) / 256;
     return static_cast<double>(rounds) * (ends + step * static_cast<double>(steps));
   }
@@ -1259,12 +1262,16 @@ template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t str
   auto by_small = [&] { hipLaunchKernelGGL((matmul_small_kernel<O, kExact, kWaves>), small.grid(), dim3(kWaves * 64), 0, stream, a, small.m, small.n); };
   auto by_split = [&] { hipLaunchKernelGGL((matmul_split_kernel<O, kExact, kWaves>), split.grid(), dim3(kWaves * 64), 0, stream, a, split.m, split.n); };
   // rows too long for the larger tiles' 32-bit offsets
-  if (a.a.ld >= (1u << 23) || a.b.ld >= (1u << 23)) return by_small();
+  if (a.a.ld >= (1u << 23) || a.b.ld >= (1u << 23)) {
+    check(small.fit(kWaves * 64), "fp8_matmul: too many values of C for rows 2^23 bytes apart");
+    return by_small();
+  }
   if constexpr (kExact) {
     // One row of A or a few, for which 16 columns to a block leave fewer CUs without one: 1 x 4096 x 4096 6.3 us
     // and 8.0 (32 x 32), 16 x 4096 x 4096 7.4 and 8.1, 16 x 8192 x 1024 11.1 and 5.7.
     if (a.m <= 16 && a.n <= 6144) return launch_rows<O, true>(a, stream);
-    const double smalls = small.time(3.8, 0.95, shared), splits = split.time(6.5, 1.95, shared), talls = tall.time(10.0, 1.75, steps);
+    const double smalls = small.time(512, 3.8, 0.95, shared), splits = split.time(512, 6.5, 1.95, shared);
+    const double talls = tall.time(512, 10.0, 1.75, steps);
     if (smalls <= std::min(splits, talls)) by_small();
     else if (splits <= talls) by_split();
     else launch_stage<O, true, 256, 128, 3>(a, stream);
@@ -1273,9 +1280,9 @@ template <class O, bool kExact> void launch(const MatmulArgs& a, hipStream_t str
     // 6.2; 1024 x 8192: 7.8 both; 1000 x 1024: 5.7 and 5.2; 8192 x 1024: 7.5 and 5.3). From 8 rows on they
     // are no faster.
     if (a.m <= 4 && a.n > 1024 && a.n <= 4096) return launch_rows<O, false>(a, stream);
-    const double smalls = small.time(2.7, 0.45, shared), splits = split.time(4.5, 0.75, shared), mids = mid.time(6.0, 0.55, steps);
-    const double highs = high.time(8.5, 0.78, steps), talls = tall.time(10.0, 0.95, steps);
-    const double bigs = a.k >= kScaleBlock ? big.time(13.0, 1.6, steps) : HUGE_VAL;  // it takes at least one whole block
+    const double smalls = small.time(256, 2.7, 0.45, shared), splits = split.time(256, 4.5, 0.75, shared), mids = mid.time(256, 6.0, 0.55, steps);
+    const double highs = high.time(384, 8.5, 0.78, steps), talls = tall.time(512, 10.0, 0.95, steps);
+    const double bigs = a.k >= kScaleBlock ? big.time(512, 13.0, 1.6, steps) : HUGE_VAL;  // it takes at least one whole block
     const double least = std::min({smalls, splits, mids, highs, talls, bigs});
     if (least == smalls) by_small();
     else if (least == splits) by_split();
@@ -1298,8 +1305,8 @@ void fp8_matmul(const MatmulArgs& a, LayerType out, hipStream_t stream) {
   check(reinterpret_cast<uintptr_t>(a.a.scales) % 4 == 0 && a.a.ld_scales % 4 == 0 &&
             reinterpret_cast<uintptr_t>(a.b.scales) % 4 == 0 && a.b.ld_scales % 4 == 0,
         "fp8: the scales of a block must start on a 4-byte boundary");
-  check(a.m <= (size_t(1) << 32) && a.n <= (size_t(1) << 32) && (a.m + 63) / 64 * ((a.n + 63) / 64) <= (size_t(1) << 24),
-        "fp8_matmul: at most 2^32 rows and columns of C, and 2^36 values");
+  check(a.m <= (size_t(1) << 32) && a.n <= (size_t(1) << 32) && (a.m + 63) / 64 * ((a.n + 63) / 64) <= (size_t(1) << 22),
+        "fp8_matmul: at most 2^32 rows and columns of C, and 2^34 values");
   switch (out) {
     case LayerType::kF32: launch<float, true>(a, stream); break;
     case LayerType::kBF16: launch<__bf16, false>(a, stream); break;

@@ -164,5 +164,11 @@ def test_native_launchers_refuse_before_launching(nat):
         nat.fp8_matmul(none, none, False, 4096, 1, 1, 1, 1, 0)
     with pytest.raises(ValueError, match="multiple of 8"):
         nat.layer_fill(4096, 12, 0)
+    near, far = (4096, 16, 4096, 1 << 20), (4096, 1 << 23, 4096, 1 << 20)
+    for out in (0, 1):
+        with pytest.raises(ValueError, match="2\\^34 values"):
+            nat.fp8_matmul(near, near, False, 4096, 1 << 20, 1 << 18, 1 << 17, 16, out)
+        with pytest.raises(ValueError, match="too many values"):
+            nat.fp8_matmul(far, near, False, 4096, 1 << 20, 1 << 17, 1 << 17, 16, out)
     with pytest.raises(ValueError, match="16-byte"):
         nat.fp8_matmul((4096, 17, 4096, 16), (4096, 16, 4096, 16), False, 4096, 1, 1, 1, 1, 0)
