@@ -1,14 +1,12 @@
-"""RCCL's gfx950 device code unpacked once per host (utils/rccl_unpack.py).
+"""The operator's own RCCL build for the fabric check (utils/rccl_unpack.py).
 
-The copy must be the installed library byte for byte outside its .hip_fatbin section, and that
-section must hold an uncompressed offload bundle with exactly the host and gfx950 entries, the
-gfx950 entry an AMDGPU code object without DWARF. A copy that is missing or keyed to another
-library is not used (the installed one is). On the MI355X the ranks load it and pass
-(tests/test_kernels_gpu.py::test_unpacked_rccl_starts_faster_on_a_real_gpu)."""
+A build that is given is kept and keyed to the installed library; one that is missing or keyed to
+another library is not used (the installed one is). The installed library itself is never opened:
+what is read here as a library is this repository's own. On the MI355X the ranks load the build where
+one is kept (tests/test_kernels_gpu.py::test_unpacked_rccl_starts_faster_on_a_real_gpu)."""
 from __future__ import annotations
 
 import json
-import struct
 from pathlib import Path
 
 import pytest
@@ -16,62 +14,6 @@ import pytest
 from tritonk8ssupervisor_amd.utils import rccl_unpack as ru
 
 pytestmark = pytest.mark.skipif(ru.installed_library() is None, reason="no librccl under ROCm")
-
-
-def _bundle_entries(f, off: int) -> list[tuple[int, int, str]]:
-    f.seek(off)
-    head = f.read(32)
-    assert head[:24] == b"__CLANG_OFFLOAD_BUNDLE__", head[:24]
-    n, = struct.unpack("<Q", head[24:32])
-    out = []
-    for _ in range(n):
-        o, s, tl = struct.unpack("<QQQ", f.read(24))
-        out.append((o, s, f.read(tl).decode()))
-    return out
-
-
-def _section_names(f, base: int) -> list[str]:
-    f.seek(base)
-    eh = f.read(64)
-    assert eh[:4] == b"\x7fELF" and struct.unpack_from("<H", eh, 0x12)[0] == 0xE0  # EM_AMDGPU
-    shoff, = struct.unpack_from("<Q", eh, 0x28)
-    shentsize, shnum, shstrndx = struct.unpack_from("<HHH", eh, 0x3A)
-    f.seek(base + shoff)
-    table = f.read(shentsize * shnum)
-    sh = [struct.unpack_from("<IIQQQQIIQQ", table, i * shentsize) for i in range(shnum)]
-    f.seek(base + sh[shstrndx][4])
-    names = f.read(sh[shstrndx][5])
-    return [names[s[0]:names.index(b"\0", s[0])].decode() for s in sh]
-
-
-@pytest.mark.timeout(600)
-def test_the_unpacked_copy_differs_only_in_its_device_code():
-    res = ru.unpack()
-    if not res["ok"]:
-        pytest.skip(res["why"])
-    src, dst = ru.installed_library(), ru.OUT / ru.LIB_NAME
-    assert ru.library_dir() == ru.OUT
-    off, size = ru.elf_section(src, ".hip_fatbin")
-    assert ru.elf_section(dst, ".hip_fatbin") == (off, size)
-    assert dst.stat().st_size == src.stat().st_size
-    with open(src, "rb") as a, open(dst, "rb") as b:
-        assert a.read(off) == b.read(off)  # headers, tables, host code before the section
-        for pos in range(off + size, src.stat().st_size, 8 << 20):  # everything after it
-            a.seek(pos)
-            b.seek(pos)
-            assert a.read(8 << 20) == b.read(8 << 20), pos
-        a.seek(off)
-        assert a.read(4) == b"CCOB"  # the installed one: compressed, every target
-        entries = _bundle_entries(b, off)
-        assert sorted(t for _, _, t in entries) == sorted([ru.HOST_TRIPLE, ru.TRIPLE])
-        o, s, _ = next(e for e in entries if e[2] == ru.TRIPLE)
-        assert o % 4096 == 0 and 0 < o + s <= size and s > (16 << 20)
-        names = _section_names(b, off + o)
-        assert ".text" in names and not any(n.startswith(".debug") for n in names)
-        b.seek(off + o + s)  # zero padding to the end of the section
-        assert b.read(min(1 << 20, size - o - s)).count(0) == min(1 << 20, size - o - s)
-    assert json.loads((ru.OUT / "stamp.json").read_text())["source"] == str(src)
-    assert ru.unpack()["changed"] is False  # current: nothing to redo
 
 
 def test_a_stale_or_disabled_copy_is_not_used(monkeypatch, tmp_path):
@@ -89,8 +31,11 @@ def test_a_stale_or_disabled_copy_is_not_used(monkeypatch, tmp_path):
     assert ru.library_dir() is None
 
 
-def test_elf_section_reader(tmp_path):
-    assert ru.elf_section(Path("/bin/sh").resolve(), ".text") is not None
+def test_elf_section_reader(tmp_path, native_build):
+    own = Path(native_build["libtk8s"])  # built here from source
+    off, size = ru.elf_section(own, ".text")
+    assert 0 < off < off + size <= own.stat().st_size
+    assert ru.elf_section(own, ".hip_fatbin") is not None and ru.elf_section(own, ".nothing") is None
     (tmp_path / "x").write_bytes(b"not an elf" * 10)
     assert ru.elf_section(tmp_path / "x", ".text") is None
 
@@ -165,14 +110,14 @@ def test_the_fabric_rank_env_passes_the_fail_fast_knobs_and_rccl_faults(monkeypa
     assert got["TK8S_FAULTS"] == "rccl.hang@sweep:1,rccl.exit@uid" and got["TK8S_GPU_SYNC_TIMEOUT_S"] == "3"
 
 
-def test_elf_section_survives_truncated_and_odd_files(tmp_path):
-    """a truncated or malformed library must not raise out of the optional unpack."""
-    sh = Path("/bin/sh").resolve().read_bytes()
-    for n in (0, 10, 64, 200, len(sh) // 2):
+def test_elf_section_survives_truncated_and_odd_files(tmp_path, native_build):
+    """A truncated or malformed library must not raise out of the optional check of a build."""
+    own = Path(native_build["libtk8s"]).read_bytes()
+    for n in (0, 10, 64, 200, len(own) // 2):
         f = tmp_path / f"t{n}"
-        f.write_bytes(sh[:n])
+        f.write_bytes(own[:n])
         ru.elf_section(f, ".hip_fatbin")  # None or a tuple; never struct.error / IndexError
-    odd = bytearray(sh[:64]) + bytes(64)
+    odd = bytearray(own[:64]) + bytes(64)
     odd[0x3C:0x3E] = (0xFFFF).to_bytes(2, "little")  # e_shnum far beyond the file
     (tmp_path / "odd").write_bytes(bytes(odd))
     assert ru.elf_section(tmp_path / "odd", ".text") is None

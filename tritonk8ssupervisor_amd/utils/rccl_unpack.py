@@ -26,8 +26,6 @@ from .build_native import ARCH, REPO, ROCM
 
 OUT = REPO / "build" / f"rccl-{ARCH}"
 LIB_NAME = "librccl.so.1"
-TRIPLE = f"hipv4-amdgcn-amd-amdhsa--{ARCH}"
-HOST_TRIPLE = "host-x86_64-unknown-linux-gnu-"
 
 
 def installed_library() -> Path | None:
