@@ -662,9 +662,9 @@ void check_out(const Fp8Matrix& m, const char* what) {
 void rms_norm_fp8(const NormArgs& a, LayerType type, LayerType weight_type, hipStream_t stream) {
   check(a.cols <= (1u << 30), "rms_norm_fp8: at most 2^30 columns");
   check(weight_type == type || weight_type == LayerType::kF32, "rms_norm_fp8: the weight is of x's type or float32");
-  if (a.rows == 0 || a.cols == 0) return;
-  check(a.x && a.weight, "rms_norm_fp8: x and weight are needed");
-  check(!a.residual || a.h, "rms_norm_fp8: a residual needs h, where the sum is stored");
+  if (a.rows == 0 || (a.cols == 0 && !a.rstd)) return;  // rows of no columns: their rstd is NaN
+  check(a.cols == 0 || (a.x && a.weight), "rms_norm_fp8: x and weight are needed");
+  check(!a.residual || a.h || a.cols == 0, "rms_norm_fp8: a residual needs h, where the sum is stored");
   check(!a.q || a.scales, "rms_norm_fp8: 8-bit values need scales");
   check(!a.q || (aligned(a.q, 16) && a.ldq % 16 == 0), "fp8: the rows of 8-bit values must start on 16-byte boundaries");
   const bool wide = weight_type == LayerType::kF32;

@@ -611,3 +611,19 @@ def test_what_a_call_returns_does_not_overlap(fp8, cols):
             (t if t.dtype == torch.float32 else t.view(torch.uint8)).fill_(85)
             for j, u in enumerate(got):
                 assert j <= i or torch.equal(bits_of(u), want[j]), (name, i, j)
+
+
+# ---- ends of ranges, and what torch may do with arguments and results ----------------------------
+
+
+@pytest.mark.parametrize("rows", [5, 30000])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_of_no_columns(fp8, rows, residual):
+    """The mean of nothing is NaN and so is rstd, whatever the memory held before."""
+    for dtype in TYPES:
+        held = [torch.full((rows,), 7.0, device="cuda") for _ in range(4)]
+        del held
+        x, w = torch.empty(rows, 0, dtype=dtype, device="cuda"), torch.empty(0, dtype=dtype, device="cuda")
+        n = fp8.rms_norm(x, w, residual=x if residual else None, normed=True)
+        assert n.values.shape == n.y.shape == n.h.shape == (rows, 0) and n.scales.shape == (rows, 0)
+        assert n.rstd.shape == (rows,) and n.rstd.isnan().all()

@@ -81,7 +81,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | 
              quantized: bool = True, normed: bool = False) -> Normed:
     """``h = x + residual`` (rounded to x's type; x itself without a residual), ``y = h / sqrt(mean(h^2) +
     eps) * weight`` for each row, as a :class:`Normed`: y in 8 bits with a scale for each 128 columns
-    of a row (``quantized``), y in x's type (``normed``), and the rows' ``1 / sqrt(...)``.
+    of a row (``quantized``), y in x's type (``normed``), and the rows' ``1 / sqrt(...)`` (NaN where there
+    are no columns).
 
     ``x``, ``residual``: rows x cols; float32, bfloat16 or float16. ``weight``: cols, of x's type or
     float32."""
