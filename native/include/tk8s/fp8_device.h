@@ -180,15 +180,29 @@ template <class T, int N> __device__ __forceinline__ void store_some(T* p, int n
   }
 }
 
-// The float nearest to zero side of v with its last bits standing for "more follows": v cut to 20
-// fraction bits, the last one set where anything was cut. Rounding the result once more, to at
-// most 18 bits, gives what rounding v itself would -- no second rounding, no false ties.
-__device__ __forceinline__ float round_to_odd(double v) {
+// The float on the zero side of v with its last bit standing for "more follows": v cut to 20 fraction bits, the
+// last one set where anything was cut. Rounding the result once more, to at most 18 bits, gives what
+// rounding v itself would -- no second rounding, no false ties. Below 2^-126 a float has fewer bits: see the next one.
+__device__ __forceinline__ unsigned odd_bits(double v) {  // the upper half of the cut v
   const unsigned long long b = __double_as_longlong(v);
-  const unsigned lo = static_cast<unsigned>(b);
-  const unsigned hi = static_cast<unsigned>(b >> 32) | (lo != 0 ? 1u : 0u);
-  return static_cast<float>(__longlong_as_double(static_cast<unsigned long long>(hi) << 32));
+  return static_cast<unsigned>(b >> 32) | (static_cast<unsigned>(b) != 0 ? 1u : 0u);
 }
+__device__ __forceinline__ float round_to_odd(double v) {
+  return static_cast<float>(__longlong_as_double(static_cast<unsigned long long>(odd_bits(v)) << 32));
+}
+
+// The same of any v: below 2^-126 it is cut to whole multiples of 2^-149, and the result can be rounded once more to
+// multiples of 2^-137 and up, which is where the borders between e4m3 values under the least scale lie.
+__device__ __forceinline__ float round_tiny_to_odd(double v) {
+  if (!(fabs(v) < 0x1p-126)) return round_to_odd(v);
+  const double steps = fabs(v) * 0x1p149;  // below 2^23, exact
+  const unsigned whole = static_cast<unsigned>(steps);
+  return __uint_as_float((odd_bits(v) & 0x80000000u) | whole | (steps != static_cast<double>(whole) ? 1u : 0u));
+}
+
+// Whether v is not 0 and below 2^-126: least <= kTiny for the least of these.
+constexpr unsigned kTiny = 0x38100000u - 2;
+__device__ __forceinline__ unsigned from_zero(double v) { return (odd_bits(v) & 0x7fffffffu) - 1; }
 
 // 1 / sqrt(x) to the last bits of 64: the instruction's first 2^-25 or so, then one step of third order.
 // 0 and infinity keep what the instruction says.

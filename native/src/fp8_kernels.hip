@@ -36,28 +36,52 @@ __device__ __forceinline__ V row_sum(V v, V* slot) {
 // RMS norm: h = x + residual rounded to T; y = h * rstd * w; the block's scale and e4m3 values
 // ------------------------------------------------------------------------------------------
 // y and its 8-bit form of 8 columns from h and the weight. y is in 32 bits, at most 3 units in the last
-// place off (v w, rstd and their product are rounded once each); where one of a wave's 512 values is
-// near enough to a border between two e4m3 values for that to matter -- one time in a hundred -- the
-// wave makes them again in 64 bits, so that every value falls where the formula puts it.
+// place off (v w, rstd and their product are rounded once each) where all three are normal numbers. Where
+// one of a wave's 512 values is near enough to a border between two e4m3 values for that to matter --
+// one time in a hundred, and wherever there is a zero: in a padded row, in lanes behind a row's end -- or
+// where a lane's values are so small that one of the three may not be normal (`low`), the wave makes
+// them again in 64 bits, so that every value falls where the formula puts it.
+//
+// A value counts in its block if it is above 2^-10 of the block's scale, 2^-19 of the block's largest. Its v w
+// is below 2^-126 only if it is below 2^-126 rstd, so blocks whose largest is 2^-107 rstd or more
+// hold none such that count; those of 2^-107 or more none whose y is below 2^-126.
+__device__ __forceinline__ unsigned low_below(float rstd32) {  // bits of the least largest magnitude that is not low
+  return __float_as_uint(rstd32 < 0x1p-126f ? __builtin_inff() : 0x1p-107f * fmaxf(rstd32, 1.f));
+}
+
 template <bool kWhole, class T, class W>
 __device__ __forceinline__ void norm_eight(const NormArgs& a, size_t row, int col, int n, const Packed8<T>& h, const Packed8<W>& w,
-                                           double rstd, float rstd32) {
+                                           double rstd, float rstd32, unsigned low) {
   float y[8];
-  unsigned least = ~0u;
+  unsigned least = ~0u, top = 0;  // columns behind the end are zeros
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     y[j] = unpack(h, j) * unpack(w, j) * rstd32;
     least = min(least, from_border(y[j]));
+    top = max(top, magnitude_bits(y[j]));
   }
-  if (__builtin_amdgcn_ballot_w64(near_border(least)) != 0 || a.y) {
+  if (__builtin_amdgcn_ballot_w64(near_border(least) || top < low) != 0 || a.y) {
     Packed8<T> o;
     float y32[8];
+    least = ~0u;
+    auto y64 = [&](int j) { return static_cast<double>(unpack(h, j)) * rstd * static_cast<double>(unpack(w, j)); };
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const double y64 = static_cast<double>(unpack(h, j)) * rstd * static_cast<double>(unpack(w, j));
-      y[j] = round_to_odd(y64);
-      y32[j] = sizeof(T) == 4 ? static_cast<float>(y64) : y[j];
+      const double v = y64(j);
+      y[j] = round_to_odd(v);
+      y32[j] = sizeof(T) == 4 ? static_cast<float>(v) : y[j];
+      least = min(least, from_zero(v));
     }
+    if (__builtin_amdgcn_ballot_w64(least <= kTiny) != 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        y[j] = round_tiny_to_odd(y64(j));
+        if (sizeof(T) == 2) y32[j] = y[j];
+      }
+    }
+    top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, magnitude_bits(y[j]));
     if (a.y) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) pack(o, j, y32[2 * j], y32[2 * j + 1]);
@@ -65,9 +89,6 @@ __device__ __forceinline__ void norm_eight(const NormArgs& a, size_t row, int co
     }
   }
   if (!a.q) return;
-  unsigned top = 0;  // columns behind the end are zeros
-#pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, magnitude_bits(y[j]));
   const unsigned byte = scale_byte(max16(top));
   store_bytes<kWhole>(a.q + row * a.ldq + col, n,
                       u32x2{pack4(y[0], y[1], y[2], y[3], byte), pack4(y[4], y[5], y[6], y[7], byte)});
@@ -144,6 +165,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(NormArg
     sum = row_sum<TPR>(sum, slot);
     const double rstd = inverse_sqrt(sum * per_col + a.eps);
     const float rstd32 = static_cast<float>(rstd);
+    const unsigned low = low_below(rstd32);
     if (live && t == 0 && a.rstd) a.rstd[row] = rstd32;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
@@ -151,7 +173,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(NormArg
       if (behind(c)) continue;
       keep_packed(sums[c]);
       keep_packed(w[c]);
-      norm_eight<kWhole>(a, row, col, live ? cols - col : 0, sums[c], w[c], rstd, rstd32);
+      norm_eight<kWhole>(a, row, col, live ? cols - col : 0, sums[c], w[c], rstd, rstd32, low);
     }
   }
 }
@@ -178,12 +200,13 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
     sum = row_sum<1024>(sum, slot);
     const double rstd = inverse_sqrt(sum * per_col + a.eps);
     const float rstd32 = static_cast<float>(rstd);
+    const unsigned low = low_below(rstd32);
     if (threadIdx.x == 0 && a.rstd) a.rstd[row] = rstd32;
     const int end = (cols + 8191) / 8192 * 8192;  // whole waves: a block's lanes look at each other
     for (int col = threadIdx.x * 8; col < end; col += 8192) {
       const Packed8<T> h = load_packed<false>((res ? static_cast<const T*>(hr) : xr) + col, cols - col);
       const Packed8<W> w = load_packed<false>(static_cast<const W*>(a.weight) + col, cols - col);
-      norm_eight<false>(a, row, col, cols - col, h, w, rstd, rstd32);
+      norm_eight<false>(a, row, col, cols - col, h, w, rstd, rstd32, low);
     }
   }
 }

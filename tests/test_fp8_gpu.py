@@ -627,3 +627,43 @@ def test_norm_of_no_columns(fp8, rows, residual):
         n = fp8.rms_norm(x, w, residual=x if residual else None, normed=True)
         assert n.values.shape == n.y.shape == n.h.shape == (rows, 0) and n.scales.shape == (rows, 0)
         assert n.rstd.shape == (rows,) and n.rstd.isnan().all()
+
+
+def tiny_case(name):
+    """(x, weight, eps) whose products, results or rstd leave the normal numbers of 32 bits."""
+    g = np.random.default_rng(11)
+    x, w = g.normal(size=(64, 17000)), np.exp2(g.uniform(-1, 1, 17000))
+    if name == "tiny products":  # h w is subnormal, y is not
+        return x * 1e-3, w * 1.5e-38, 1e-12
+    if name == "vanishing products":  # h w is 0 in 32 bits
+        return x * 1e-12, w * 1e-36, 1e-28
+    if name == "tiny results":
+        return x, w * 1e-39, 1e-6
+    if name == "tiny products beside large ones":  # blocks of either kind in one wave
+        return x * 1e-3, np.where(np.arange(17000) // 128 % 2 == 0, w, w * 1.5e-38), 1e-12
+    if name == "tiny rstd":
+        return x * 3e37, w * 1e-3, 1e-6
+    if name == "small rows":  # rstd is beyond 32 bits
+        return x * 1e-39, w, 0.0
+    assert name == "tiny rows"
+    return x * 1e-41, w, 0.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [1000, 104, 200, 600, 17000])
+@pytest.mark.parametrize("name", ["tiny products", "vanishing products", "tiny results", "tiny products beside large ones", "tiny rstd", "small rows", "tiny rows"])
+def test_norm_at_the_ends_of_32_bits(fp8, name, cols, dtype):
+    x, w, eps = tiny_case(name)
+    x, w = torch.from_numpy(x[:, :cols].copy()).to(dtype), torch.from_numpy(w[:cols].copy())
+    w = w.to(torch.float32 if dtype == torch.float16 else dtype)
+    x[3], x[5, 7:20] = 0, 0
+    n = fp8.rms_norm(x.cuda(), w.cuda(), eps=eps)
+    with np.errstate(divide="ignore", invalid="ignore"):  # a row of zeros whose eps is 0 is NaN
+        y, _ = ref.rms_norm(x.double().numpy(), w.double().numpy(), eps)
+    q, s = ref.fp8_quantize(y)
+    np.testing.assert_array_equal(bits(n.scales), s)
+    np.testing.assert_array_equal(host(n.values), ref.e4m3_values()[q])
+    rows = np.isfinite(y).all(axis=1)
+    full = fp8.rms_norm(x.cuda(), w.cuda(), eps=eps, normed=True)
+    np.testing.assert_array_equal(bits(full.values), bits(n.values))
+    close(host(full.y)[rows], y[rows], 1.0001 * HALF[dtype] * np.abs(y[rows]) + 1.0001 * TINY[dtype])
