@@ -415,9 +415,13 @@ template <class F, class O> __device__ __forceinline__ void sum_columns(size_t r
   }
 }
 
+constexpr size_t kSumBlocks = size_t(1) << 20;  // at most: a launch has fewer than 2^32 threads
+
 __global__ __launch_bounds__(1024) void column_sum_kernel(const float* part, size_t rows, size_t cols, float* dw) {
-  sum_columns(rows, cols, static_cast<size_t>(blockIdx.x) * kSumCols, [&](size_t r, size_t c) { return part[r * cols + c]; },
-              [&](size_t c, float s) { dw[c] = s; });
+  for (size_t col0 = static_cast<size_t>(blockIdx.x) * kSumCols; col0 < cols; col0 += static_cast<size_t>(gridDim.x) * kSumCols) {
+    sum_columns(rows, cols, col0, [&](size_t r, size_t c) { return part[r * cols + c]; }, [&](size_t c, float s) { dw[c] = s; });
+    __syncthreads();  // the slices have been read
+  }
 }
 
 // Few rows: one launch. The first blocks make dx, a row each; the others dw, kSumCols columns each, from dy and
@@ -502,7 +506,7 @@ template <class T, class W> void launch_backward(const NormBackwardArgs& a, hipS
     if (a.cols % 8 == 0) launch_backward_rows<T, W, true>(a, grid, stream);
     else launch_backward_rows<T, W, false>(a, grid, stream);
     TK8S_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(column_sum_kernel, dim3(static_cast<unsigned>(sums)), dim3(1024), 0, stream, a.workspace,
+    hipLaunchKernelGGL(column_sum_kernel, dim3(static_cast<unsigned>(std::min(sums, kSumBlocks))), dim3(1024), 0, stream, a.workspace,
                        static_cast<size_t>(grid), a.cols, a.dw);
   }
   TK8S_HIP_CHECK(hipGetLastError());

@@ -667,3 +667,22 @@ def test_norm_at_the_ends_of_32_bits(fp8, name, cols, dtype):
     full = fp8.rms_norm(x.cuda(), w.cuda(), eps=eps, normed=True)
     np.testing.assert_array_equal(bits(full.values), bits(n.values))
     close(host(full.y)[rows], y[rows], 1.0001 * HALF[dtype] * np.abs(y[rows]) + 1.0001 * TINY[dtype])
+
+
+def test_norm_backward_of_rows_that_fill_a_launch(fp8):
+    """2^27 columns and some: 32 columns to a block of 1024 threads would be 2^32 threads."""
+    rows, cols = 2, (1 << 27) + 40
+    i = torch.arange(cols, device="cuda")
+    h = torch.stack([i % 251 - 125, i % 127 - 63]).bfloat16()
+    dy = torch.stack([i % 61 - 30, i % 113 - 56]).bfloat16()
+    w, rstd = (i % 5 + 1).bfloat16(), torch.tensor([0.5, 0.25], device="cuda")
+    dx, dw = fp8.rms_norm_backward(dy, h, w, rstd)
+    want = (dy.float() * h.float() * rstd[:, None]).sum(0)  # every product and sum is exact in 32 bits
+    assert torch.equal(dw, want)
+    del want
+    part = slice(cols - 1000, cols)
+    mean = torch.stack([(dy[r].float() * w.float() * h[r].float()).sum(dtype=torch.float64) * rstd[r] / cols for r in range(rows)])
+    g, xh = (dy[:, part].double() * w[part].double()), h[:, part].double() * rstd[:, None]
+    want = rstd[:, None] * (g - xh * mean[:, None])
+    size = rstd[:, None] * (4 * g.abs() + xh.abs() * 30 * 5 * 63)  # a sum over 2^27 in 1024 threads: (2^17 + 30) roundings of the mean's parts
+    assert ((dx[:, part].double() - want).abs() <= HALF[torch.bfloat16] * want.abs() + (2.0 ** 17 + 30) * U * size).all()
