@@ -6,6 +6,7 @@
 //  * raw launchers (hbm_fill, philox_fill, md5_tree, ar_fill, ar_check, stream_copy): take
 //    device pointers and a hipStream_t as integers (e.g. torch tensor.data_ptr() and
 //    torch.cuda.current_stream().cuda_stream) — what the numerics tests use.
+#include <pybind11/numpy.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
@@ -39,6 +40,8 @@ tk8s::LayerType layer_type_of(int t) {
   return static_cast<tk8s::LayerType>(t);
 }
 
+template <class T> using Array = py::array_t<T, py::array::c_style | py::array::forcecast>;
+
 // (values, row pitch, scales, scale pitch); zeros: not asked for
 using Fp8Tuple = std::tuple<uintptr_t, size_t, uintptr_t, size_t>;
 tk8s::Fp8Matrix fp8_of(const Fp8Tuple& t) {
@@ -65,6 +68,21 @@ PYBIND11_MODULE(_tk8s_native, m) {
         py::arg("bytes"), py::arg("iters") = 10, py::arg("dma") = true, G());
   m.def("layer_probe", &tk8s::layer_probe, py::arg("rows") = 4096, py::arg("width") = 4096, py::arg("seed") = 0,
         py::arg("iters") = 3, py::arg("device") = 0, G());
+  // the layer probe's host checks on numpy arrays (bf16 as uint16)
+  m.def(
+      "layer_rounding_error",
+      [](const Array<uint16_t>& source, const Array<uint8_t>& values, uint8_t scale) {
+        if (source.size() != values.size()) throw std::invalid_argument("as many values as were rounded");
+        return tk8s::layer_rounding_error(source.data(), values.data(), static_cast<size_t>(source.size()), scale);
+      },
+      py::arg("source"), py::arg("values"), py::arg("scale"));
+  m.def(
+      "layer_weight_sum_error",
+      [](float got, const Array<uint16_t>& dy, const Array<uint16_t>& h, const Array<float>& rstd) {
+        if (dy.size() != h.size() || dy.size() != rstd.size()) throw std::invalid_argument("dy, h and rstd must have as many rows");
+        return tk8s::layer_weight_sum_error(got, dy.data(), h.data(), rstd.data(), static_cast<size_t>(dy.size()));
+      },
+      py::arg("got"), py::arg("dy"), py::arg("h"), py::arg("rstd"));
   m.def(
       "rccl_allreduce",
       [](const std::vector<int>& devices, size_t min_bytes, size_t max_bytes, int factor,

@@ -33,10 +33,17 @@ std::string copy_probe(int src_device, int dst_device, size_t bytes, int iters, 
 // Matrix cores: one step of an 8-bit layer, forward and backward, on rows x width activations and a
 // width x width weight (multiples of 128, up to 16384) made from the seed: a norm after a residual, rounding to
 // 8 bits, y = x W^T, the gradients of x and W, and the norm's. Sampled rows are computed again on the
-// host in 64 bits ("error": the largest, as a share of what rounding allows; above 1 is a failure), and
+// host in 64 bits ("error": the largest, as a share of what rounding allows; above 1 is a failure;
+// "compared": of how many values), in each of the three layouts of rounded values byte for byte, and
 // the MD5 tree of everything that came out ("digest") has to be the same in each of the `iters` steps;
 // so must it be on every device. Reports the products' TFLOP/s and the other kernels' GB/s.
 std::string layer_probe(size_t rows, size_t width, uint64_t seed, int iters, int device);
+
+// Two of its host checks, as shares of what is allowed (0: equal): n e4m3 values that share an E8M0 scale against the
+// bf16 values that they were rounded from, where every byte is given; one value of the norm's weight gradient
+// against sum(dy * h * rstd) over the rows of its column.
+double layer_rounding_error(const uint16_t* source, const uint8_t* values, size_t n, uint8_t scale);
+double layer_weight_sum_error(float got, const uint16_t* dy, const uint16_t* h, const float* rstd, size_t rows);
 
 // The local probes share one grow-on-demand device allocation per device (see probes.cpp);
 // free them (e.g. from a long-lived process once validation is done).

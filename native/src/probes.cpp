@@ -532,16 +532,27 @@ double bf16_value(uint16_t v) {
   return f;
 }
 
-double e4m3_value(uint8_t v) {
+double e4m3_of(uint8_t v) {
   const int e = v >> 3 & 15, m = v & 7;
   if (e == 15 && m == 7) return std::nan("");
   const double x = e ? std::ldexp(8 + m, e - 10) : std::ldexp(m, -9);
   return v & 128 ? -x : x;
 }
 
+double e4m3_value(uint8_t v) {
+  static const std::vector<double> table = [] {
+    std::vector<double> t(256);
+    for (int i = 0; i < 256; ++i) t[i] = e4m3_of(static_cast<uint8_t>(i));
+    return t;
+  }();
+  return table[v];
+}
+
 struct Compared {
   double worst = 0;  // the largest error so far, as a share of the allowed one
+  uint64_t count = 0;
   void add(double got, double want, double allowed) {
+    ++count;
     const double e = std::fabs(got - want);
     worst = std::max(worst, e <= allowed ? (allowed > 0 ? e / allowed : 0.0) : (e == e && allowed > 0 ? e / allowed : 1e30));
   }
@@ -556,6 +567,14 @@ std::vector<double> fetch_row(const Fp8Matrix& m, size_t r, size_t scale_row, si
   std::vector<double> x(k);
   for (size_t i = 0; i < k; ++i) x[i] = sc[i / 128] == 255 ? std::nan("") : std::ldexp(e4m3_value(v[i]), sc[i / 128] - 127);
   return x;
+}
+
+// `height` pieces of `n` values each, `pitch` bytes apart.
+template <class T> std::vector<T> fetch_raw(const void* p, size_t n, size_t pitch, size_t height, hipStream_t s) {
+  std::vector<T> v(n * height);
+  TK8S_HIP_CHECK(hipMemcpy2DAsync(v.data(), n * sizeof(T), p, pitch, n * sizeof(T), height, hipMemcpyDeviceToHost, s));
+  wait_stream(s, "layer probe");
+  return v;
 }
 
 template <class T> std::vector<double> fetch(const void* p, size_t n, hipStream_t s) {  // 16-bit or 32-bit values
@@ -589,7 +608,57 @@ void compare_dot(Compared& c, double got, const std::vector<double>& x, const st
   c.add(got, want, off);
 }
 
+// The E8M0 byte of a block of this largest magnitude: the least power of two that brings it to 448 or below.
+int scale_byte_of(double top) {
+  if (top == 0) return 127;
+  int e = 0;
+  const double m = std::frexp(top, &e);
+  return std::clamp(e - (m <= 0.875 ? 9 : 8), -127, 127) + 127;
+}
+
+// Values in 8 bits that share a scale against the 16-bit ones that they were made of: every byte is given.
+void compare_rounded(Compared& c, const uint16_t* source, const uint8_t* values, size_t n, uint8_t scale) {
+  double top = 0;
+  for (size_t i = 0; i < n; ++i) top = std::max(top, std::fabs(bf16_value(source[i])));
+  const int byte = scale_byte_of(top);
+  c.add(scale, byte, 0);
+  const double by = std::ldexp(1.0, 127 - byte);
+  for (size_t i = 0; i < n; ++i) {
+    const double v = bf16_value(source[i]) * by, size = std::fabs(v);
+    uint64_t binade;  // of the power of two at or below it
+    std::memcpy(&binade, &size, 8);
+    binade &= uint64_t(0x7ff) << 52;
+    double power;
+    std::memcpy(&power, &binade, 8);
+    const double step = std::max(power, 0x1p-6) / 8;
+    c.add(e4m3_value(values[i]), std::nearbyint(v / step) * step, 0);
+  }
+}
+
+// One value of the norm's weight gradient against its sum in 64 bits: rows + 4 roundings of 32-bit sums.
+void compare_weight_sum(Compared& c, double got, const uint16_t* dy, const uint16_t* h, const float* rstd, size_t rows) {
+  double want = 0, size = 0;
+  for (size_t r = 0; r < rows; ++r) {
+    const double p = bf16_value(dy[r]) * bf16_value(h[r]) * rstd[r];
+    want += p;
+    size += std::fabs(p);
+  }
+  c.add(got, want, static_cast<double>(rows + 4) * std::ldexp(size, -24));
+}
+
 }  // namespace
+
+double layer_rounding_error(const uint16_t* source, const uint8_t* values, size_t n, uint8_t scale) {
+  Compared c;
+  compare_rounded(c, source, values, n, scale);
+  return c.worst;
+}
+
+double layer_weight_sum_error(float got, const uint16_t* dy, const uint16_t* h, const float* rstd, size_t rows) {
+  Compared c;
+  compare_weight_sum(c, got, dy, h, rstd, rows);
+  return c.worst;
+}
 
 std::string layer_probe(size_t rows, size_t width, uint64_t seed, int iters, int device) {
   try {
@@ -610,6 +679,7 @@ std::string layer_probe(size_t rows, size_t width, uint64_t seed, int iters, int
     const size_t o_out = at;  // what the digest is taken of: y W^T, then the gradients
     const size_t o_c = place(2 * n), o_dx = place(2 * n), o_dw = place(4 * width * width), o_dnw = place(4 * width), out_bytes = at - o_out;
     const size_t tree = md5_tree_workspace(out_bytes, 1024), o_wa = place(tree), o_wb = place(tree), o_md = place(16);
+    const size_t o_col = place(2 * std::max(rows, width));
     char* const base = scratch(device, at);
     auto u8 = [&](size_t o) { return reinterpret_cast<uint8_t*>(base + o); };
     const Fp8Matrix q{u8(o_q), width, u8(o_qs), rows}, yc{u8(o_yc), rows, u8(o_ycs), width}, wt{u8(o_wt), width, u8(o_wts), tiles},
@@ -669,6 +739,7 @@ std::string layer_probe(size_t rows, size_t width, uint64_t seed, int iters, int
     // sampled rows and columns again on the host
     Compared norm, rounding, forward, input, weight, backward;
     const std::vector<double> nw = fetch<uint16_t>(base + o_nw, width, st.s);
+    const std::vector<float> rstds = fetch_raw<float>(base + o_rstd, rows, 4 * rows, 1, st.s);
     constexpr size_t kSamples = 12;
     auto sample = [](size_t i, size_t count) { return (i * (count - 1) / (kSamples - 1) + 37 * i) % count; };
     std::vector<std::vector<double>> w_rows, wc_rows, yc_rows;
@@ -678,8 +749,32 @@ std::string layer_probe(size_t rows, size_t width, uint64_t seed, int iters, int
       wc_rows.push_back(fetch_row(wc, col, col, width, st.s));
       yc_rows.push_back(fetch_row(yc, col, col, rows, st.s));
     }
+    // what the roundings made of their 16-bit values: a row of the first layout, a column of the transposed ones, a tile
+    auto check_blocks = [&](const std::vector<uint16_t>& source, const Fp8Matrix& m, size_t r) {
+      const auto v = fetch_raw<uint8_t>(m.values + r * m.ld, source.size(), source.size(), 1, st.s);
+      const auto sc = fetch_raw<uint8_t>(m.scales + r, 1, m.ld_scales, source.size() / 128, st.s);
+      for (size_t b = 0; b < sc.size(); ++b) compare_rounded(rounding, &source[b * 128], &v[b * 128], 128, sc[b]);
+    };
+    auto column = [&](size_t of, size_t col, size_t count) {  // put together on the device: the host would fetch it value by value
+      TK8S_HIP_CHECK(hipMemcpy2DAsync(base + o_col, 2, base + of + 2 * col, 2 * width, 2, count, hipMemcpyDeviceToDevice, st.s));
+      return fetch_raw<uint16_t>(base + o_col, count, 2 * count, 1, st.s);
+    };
+    for (size_t i = 0; i < kSamples; ++i) {
+      const size_t r = sample(i, rows), col = sample(i, width), tile_r = sample(i, blocks), tile_c = (tile_r + 5 * i) % blocks;
+      check_blocks(fetch_raw<uint16_t>(base + o_g + 2 * r * width, width, 2 * width, 1, st.s), gr, r);
+      check_blocks(column(o_g, col, rows), gc, col);
+      check_blocks(column(o_y, col, rows), yc, col);
+      check_blocks(column(o_w, col, width), wc, col);
+      const auto source = fetch_raw<uint16_t>(base + o_w + 2 * 128 * (tile_r * width + tile_c), 128, 2 * width, 128, st.s);
+      const auto tile = fetch_raw<uint8_t>(wt.values + 128 * (tile_r * width + tile_c), 128, width, 128, st.s);
+      compare_rounded(rounding, source.data(), tile.data(), 128 * 128,
+                      fetch_raw<uint8_t>(wt.scales + tile_c * wt.ld_scales + tile_r, 1, 1, 1, st.s)[0]);
+      compare_weight_sum(backward, fetch_raw<float>(base + o_dnw + 4 * col, 1, 4, 1, st.s)[0], column(o_dq, col, rows).data(),
+                         column(o_h, col, rows).data(), rstds.data(), rows);
+    }
     for (size_t i = 0; i < kSamples; ++i) {
       const size_t r = sample(i, rows);
+      const auto q_scales = fetch_raw<uint8_t>(q.scales + r, 1, q.ld_scales, blocks, st.s);
       const auto x = fetch<uint16_t>(base + o_x + 2 * r * width, width, st.s), res = fetch<uint16_t>(base + o_res + 2 * r * width, width, st.s);
       const auto h = fetch<uint16_t>(base + o_h + 2 * r * width, width, st.s), y = fetch<uint16_t>(base + o_y + 2 * r * width, width, st.s);
       const auto qr = fetch_row(q, r, r, width, st.s), gq = fetch_row(gr, r, r, width, st.s);
@@ -688,6 +783,7 @@ std::string layer_probe(size_t rows, size_t width, uint64_t seed, int iters, int
       double squares = 0, along = 0, along_size = 0;
       for (double v : h) squares += v * v;
       const double rstd = 1 / std::sqrt(squares / static_cast<double>(width) + 1e-5);
+      norm.add(rstds[r], rstd, std::ldexp(rstd, -24) * (1 + 1e-6));
       const double sums = static_cast<double>(width + 8) * std::ldexp(1.0, -24);  // of 32-bit sums, relative to their size
       for (size_t j = 0; j < width; ++j) {
         const double want = h[j] * rstd * nw[j];
@@ -697,6 +793,8 @@ std::string layer_probe(size_t rows, size_t width, uint64_t seed, int iters, int
         double top = 0;
         for (size_t b = j / 128 * 128; b < j / 128 * 128 + 128; ++b) top = std::max(top, std::fabs(h[b] * rstd * nw[b]));
         rounding.add(qr[j], want, (std::ldexp(std::fabs(want), -4) + std::ldexp(top / 224, -10)) * (1 + 1e-6));
+        // its scale, too, unless the host's last bits decide between two
+        if (j % 128 == 0 && scale_byte_of(top * (1 - 1e-9)) == scale_byte_of(top * (1 + 1e-9))) rounding.add(q_scales[j / 128], scale_byte_of(top), 0);
         along += dq[j] * nw[j] * h[j];
         along_size += std::fabs(dq[j] * nw[j] * h[j]);
       }
@@ -734,6 +832,8 @@ std::string layer_probe(size_t rows, size_t width, uint64_t seed, int iters, int
         .kv("error", worst)
         .raw("errors", Json().kv("norm", norm.worst).kv("rounding", rounding.worst).kv("forward", forward.worst)
                            .kv("input_gradient", input.worst).kv("weight_gradient", weight.worst).kv("norm_gradient", backward.worst).str())
+        .raw("compared", Json().kv("norm", norm.count).kv("rounding", rounding.count).kv("forward", forward.count)
+                             .kv("input_gradient", input.count).kv("weight_gradient", weight.count).kv("norm_gradient", backward.count).str())
         .kv("ms", total)
         .kv("forward_tflops", rate(flops, ms[kForward], 1e12))
         .kv("input_gradient_tflops", rate(flops, ms[kInput], 1e12))

@@ -48,3 +48,68 @@ def test_setup_passes_it_on(tmp_path, monkeypatch):
     s = orchestrator.Setup(orchestrator.Workspace(tmp_path), layer=True)
     assert "--layer" in s._validation_command()
     assert "--layer" not in orchestrator.Setup(orchestrator.Workspace(tmp_path))._validation_command()
+
+
+# ---- its checks on the host, and mistakes planted in what they are given ------------------------------
+
+
+@pytest.fixture(scope="module")
+def nat(native_build):
+    from tritonk8ssupervisor_amd.ops import native
+
+    return native()
+
+
+def _bf16(x):
+    import numpy as np
+
+    u = np.asarray(x, dtype=np.float32).view(np.uint32)
+    return ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)  # to nearest, ties to even
+
+
+def _value(u):
+    import numpy as np
+
+    return (u.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+
+
+@pytest.mark.parametrize("n", [128, 128 * 128])
+@pytest.mark.parametrize("spread", [1.0, 1e-30, 1e36, 0.0])
+def test_rounded_values_are_held_to_every_byte(nat, n, spread):
+    import numpy as np
+
+    from tritonk8ssupervisor_amd.ops import reference as ref
+
+    rng = np.random.default_rng(n)
+    source = _bf16(rng.normal(size=n) * spread)
+    source[:64] = _bf16(np.arange(-32, 32) / 32 * spread)  # ties among them
+    values, scales = ref.fp8_quantize(_value(source).reshape(n // 128, 128), block_rows=n // 128)
+    values, scale = values.ravel(), int(scales[0, 0])
+    assert nat.layer_rounding_error(source, values, scale) == 0
+    for wrong in (scale - 1, scale + 1):
+        assert nat.layer_rounding_error(source, values, wrong) > 1
+    for at, mask in ((0, 1), (n // 2, 1), (n - 1, 8), (n - 1, 0x7F)):
+        planted = values.copy()
+        planted[at] ^= mask
+        assert nat.layer_rounding_error(source, planted, scale) > 1, (at, mask)
+    other = values.copy()
+    other[[1, 40]] = other[[40, 1]]
+    assert spread == 0 or nat.layer_rounding_error(source, other, scale) > 1
+    with pytest.raises(ValueError):
+        nat.layer_rounding_error(source, values[:-1], scale)
+
+
+@pytest.mark.parametrize("rows", [128, 4096])
+def test_the_norms_weight_gradient_is_held_to_its_sum(nat, rows):
+    import numpy as np
+
+    rng = np.random.default_rng(rows)
+    dy, h = _bf16(rng.normal(size=rows)), _bf16(rng.normal(size=rows) * 3)
+    rstd = rng.uniform(0.2, 1, rows).astype(np.float32)
+    terms = _value(dy) * _value(h) * rstd
+    want, allowed = terms.sum(), (rows + 4) * 2.0 ** -24 * np.abs(terms).sum()
+    assert nat.layer_weight_sum_error(np.float32(want), dy, h, rstd) <= 1
+    for planted in (want + 2 * allowed, want - 2 * allowed, want + np.abs(terms).sum() / 100, float("nan")):
+        assert nat.layer_weight_sum_error(np.float32(planted), dy, h, rstd) > 1, planted
+    with pytest.raises(ValueError):
+        nat.layer_weight_sum_error(0.0, dy, h, rstd[:-1])

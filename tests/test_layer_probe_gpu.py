@@ -72,3 +72,15 @@ def test_the_tool_reports_it(nat):
     assert p.returncode == 1 and not r["ok"] and not r["devices"][0]["ok"]
     p = subprocess.run([str(tool("tk8s-probe")), *small], capture_output=True, text=True, timeout=100)
     assert p.returncode == 0 and "layer" not in json.loads(p.stdout) and "layer" not in json.loads(p.stdout)["devices"][0]["phase_ms"]
+
+
+@pytest.mark.parametrize("rows,width", [(128, 256), (1152, 1024)])
+def test_it_compares_everything_that_a_step_makes(nat, rows, width):
+    """Of 12 sampled rows and columns each: h, y and rstd; the norm's 8-bit row with its scales, the gradient's row and
+    column, y's and the weight's columns and a tile of the weight, byte for byte; the products; dx and the norm's dw."""
+    r = json.loads(nat.layer_probe(rows, width, 3, 1, 0))
+    assert r["ok"], r
+    blocks = lambda n: n + n // 128  # values and their scales
+    assert r["compared"] == {"norm": 12 * (2 * width + 1), "forward": 144, "input_gradient": 144, "weight_gradient": 144,
+                             "norm_gradient": 12 * (width + 1),
+                             "rounding": 12 * (2 * blocks(width) + 2 * blocks(rows) + blocks(width) + 128 * 128 + 1)}
