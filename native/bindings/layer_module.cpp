@@ -7,7 +7,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <ATen/hip/EmptyTensor.h>
+#include <ATen/EmptyTensor.h>
+#include <ATen/hip/HIPContextLight.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -96,40 +97,16 @@ class Device {
     stream_ = c10::hip::getCurrentHIPStream(device_.index()).stream();
   }
   hipStream_t stream() const { return stream_; }
-  Tensor empty(at::IntArrayRef sizes, ScalarType type) const { return at::detail::empty_cuda(sizes, type, device_, std::nullopt); }
+  // A tensor with memory of its own, from torch's allocator for the device that is current here. (The general
+  // way looks for the device again: 0.2 us for each of the four results of a norm of one token, which takes 5.)
+  Tensor empty(at::IntArrayRef sizes, ScalarType type) const {
+    return at::detail::empty_generic(sizes, at::cuda::getCUDADeviceAllocator(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+  }
 
  private:
   c10::Device device_;
   std::optional<c10::DeviceGuard> guard_;
   hipStream_t stream_ = nullptr;
-};
-
-// The tensors a call returns, `bytes` in all. Up to 64 KB they share one allocation (and live as long as the
-// last of them): each of its own costs the host 0.3 us, where a call on one token takes 5 (the norm's
-// four: 5.9 -> 4.9 us; the rounding's two: 4.8 -> 4.5).
-class Room {
- public:
-  Room(const Device& dev, int64_t bytes) : dev_(dev), bytes_(bytes) {
-    if (bytes <= (64 << 10)) all_ = dev.empty({bytes}, ScalarType::Byte);
-  }
-  static int64_t bytes(int64_t values, ScalarType type) { return up(values * static_cast<int64_t>(c10::elementSize(type)), kAlign); }
-  Tensor empty(at::IntArrayRef sizes, ScalarType type) {
-    if (!all_.defined()) return dev_.empty(sizes, type);
-    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all_.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
-                                                        c10::scalarTypeToTypeMeta(type));
-    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-    t.unsafeGetTensorImpl()->set_storage_offset(next_ / static_cast<int64_t>(c10::elementSize(type)));
-    next_ += bytes(t.numel(), type);
-    TORCH_INTERNAL_ASSERT(next_ <= bytes_);
-    return t;
-  }
-
- private:
-  static constexpr int64_t kAlign = 256;
-  const Device& dev_;
-  const int64_t bytes_;
-  int64_t next_ = 0;
-  Tensor all_;
 };
 
 // Room for rows x cols values in 8 bits and for the scales of scale_rows rows (or tiles), block by block.
@@ -141,13 +118,9 @@ struct Packed {
 };
 
 int64_t pitch_of(int64_t cols) { return up(cols, cols > 512 ? 128 : 16); }
-int64_t packed_bytes(int64_t rows, int64_t cols, int64_t scale_rows) {
-  return Room::bytes(rows * pitch_of(cols), ScalarType::Byte) + Room::bytes(blocks_of(cols) * up(scale_rows, 16), ScalarType::Byte);
-}
-
-Packed packed(Room& room, int64_t rows, int64_t cols, int64_t scale_rows) {
+Packed packed(const Device& dev, int64_t rows, int64_t cols, int64_t scale_rows) {
   const int64_t ld = pitch_of(cols), lds = up(scale_rows, 16), blocks = blocks_of(cols);
-  Packed p{room.empty({rows, ld}, ScalarType::Float8_e4m3fn), room.empty({blocks, lds}, ScalarType::Float8_e8m0fnu)};
+  Packed p{dev.empty({rows, ld}, ScalarType::Float8_e4m3fn), dev.empty({blocks, lds}, ScalarType::Float8_e8m0fnu)};
   p.at = {static_cast<uint8_t*>(p.values.data_ptr()), static_cast<size_t>(ld), static_cast<uint8_t*>(p.scales.data_ptr()),
           static_cast<size_t>(lds)};
   p.values.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({rows, cols}), at::IntArrayRef({ld, 1}));
@@ -181,13 +154,10 @@ PyObject* quantize(PyObject* const* args, Py_ssize_t nargs) {
   const int64_t rows = x.size(0), cols = x.size(1);
   const Device dev({&x});
   tk8s::QuantizeArgs a{x.data_ptr(), pitch(&x), static_cast<size_t>(rows), static_cast<size_t>(cols), {}, {}, {}};
-  Room room(dev, (layout == 0 || layout == 2 ? packed_bytes(rows, cols, rows) : 0) +
-                     (layout == 1 || layout == 2 ? packed_bytes(cols, rows, cols) : 0) +
-                     (layout == 3 ? packed_bytes(rows, cols, blocks_of(rows)) : 0));
   Packed p, q;
-  if (layout == 0 || layout == 2) p = packed(room, rows, cols, rows), a.rows_out = p.at;
-  if (layout == 1 || layout == 2) q = packed(room, cols, rows, cols), a.cols_out = q.at;
-  if (layout == 3) p = packed(room, rows, cols, blocks_of(rows)), a.tiles_out = p.at;
+  if (layout == 0 || layout == 2) p = packed(dev, rows, cols, rows), a.rows_out = p.at;
+  if (layout == 1 || layout == 2) q = packed(dev, cols, rows, cols), a.cols_out = q.at;
+  if (layout == 3) p = packed(dev, rows, cols, blocks_of(rows)), a.tiles_out = p.at;
   tk8s::fp8_quantize(a, type, dev.stream());
   if (layout == 2) return tuple_of({&p.values, &p.scales, &q.values, &q.scales});
   return layout == 1 ? tuple_of({&q.values, &q.scales}) : tuple_of({&p.values, &p.scales});
@@ -206,14 +176,11 @@ PyObject* rms_norm(PyObject* const* args, Py_ssize_t nargs) {
   if (!(eps >= 0.0)) wrong_value("eps must not be negative, but is ", eps);
   const bool quantized = args[4] == Py_True, normed = args[5] == Py_True;
   const Device dev({&x, &weight, residual});
-  const int64_t matrix_bytes = Room::bytes(rows * cols, x.scalar_type());
-  Room room(dev, (residual ? matrix_bytes : 0) + (quantized ? packed_bytes(rows, cols, rows) : 0) + (normed ? matrix_bytes : 0) +
-                     Room::bytes(rows, ScalarType::Float));
-  Tensor h = residual ? room.empty({rows, cols}, x.scalar_type()) : x, y;
+  Tensor h = residual ? dev.empty({rows, cols}, x.scalar_type()) : x, y;
   Packed p;
-  if (quantized) p = packed(room, rows, cols, rows);
-  if (normed) y = room.empty({rows, cols}, x.scalar_type());
-  Tensor rstd = room.empty({rows}, ScalarType::Float);
+  if (quantized) p = packed(dev, rows, cols, rows);
+  if (normed) y = dev.empty({rows, cols}, x.scalar_type());
+  Tensor rstd = dev.empty({rows}, ScalarType::Float);
   const size_t ld = static_cast<size_t>(cols);
   tk8s::rms_norm_fp8({x.data_ptr(), pitch(&x), data<const void>(residual), pitch(residual), weight.data_ptr(),
                       residual ? h.data_ptr() : nullptr, ld, p.at.values, p.at.ld, p.at.scales, p.at.ld_scales,
@@ -233,13 +200,12 @@ PyObject* rms_norm_backward(PyObject* const* args, Py_ssize_t nargs) {
   const Tensor& weight = vector(args[2], "weight", cols, h.scalar_type());
   const Tensor& rstd = vector(args[3], "rstd", rows, ScalarType::Float);
   const Device dev({&h, &dy, &weight, &rstd, dh});
-  Room room(dev, Room::bytes(rows * cols, h.scalar_type()) + Room::bytes(cols, ScalarType::Float));
-  Tensor dx = room.empty({rows, cols}, h.scalar_type());
+  Tensor dx = dev.empty({rows, cols}, h.scalar_type());
   if (rows == 0 || cols == 0) {
     Tensor none = at::zeros({cols}, h.options().dtype(ScalarType::Float));
     return tuple_of({&dx, &none});
   }
-  Tensor dw = room.empty({cols}, ScalarType::Float), work;
+  Tensor dw = dev.empty({cols}, ScalarType::Float), work;
   const size_t n = static_cast<size_t>(rows), ld = static_cast<size_t>(cols);
   const size_t work_bytes = tk8s::rms_norm_backward_workspace(n, ld);
   if (work_bytes) work = dev.empty({static_cast<int64_t>(work_bytes)}, ScalarType::Byte);

@@ -686,3 +686,17 @@ def test_norm_backward_of_rows_that_fill_a_launch(fp8):
     want = rstd[:, None] * (g - xh * mean[:, None])
     size = rstd[:, None] * (4 * g.abs() + xh.abs() * 30 * 5 * 63)  # a sum over 2^27 in 1024 threads: (2^17 + 30) roundings of the mean's parts
     assert ((dx[:, part].double() - want).abs() <= HALF[torch.bfloat16] * want.abs() + (2.0 ** 17 + 30) * U * size).all()
+
+
+@pytest.mark.parametrize("cols", [200, 4096])
+def test_what_a_call_returns_can_be_resized_and_saved_alone(fp8, cols):
+    """Every result has memory of its own: growing one moves it, and leaves the others."""
+    x, w = torch.randn(3, cols, device="cuda"), torch.randn(cols, device="cuda")
+    n = fp8.rms_norm(x, w, residual=x, normed=True)
+    for got in ([n.h, n.values, n.scales, n.y, n.rstd], [t for q in fp8.quantize(x, layout="both") for t in q],
+                list(fp8.quantize(x, layout="tiles")), list(fp8.rms_norm_backward(x, n.h, w, n.rstd))):
+        want = [bits_of(t).clone() for t in got]
+        for i, t in enumerate(got):
+            t.resize_(64, cols).view(torch.uint8).fill_(85)
+            for j, u in enumerate(got):
+                assert j <= i or torch.equal(bits_of(u), want[j]), (i, j)

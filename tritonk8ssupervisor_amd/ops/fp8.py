@@ -16,8 +16,7 @@ block of zeros); values round to nearest even. A block that holds a NaN or an in
 Sums are in 32 bits or more and rounded once. The same inputs give the same bits on every call.
 
 Every call is asynchronous on the current stream of its tensors' device, allocates only what it
-returns and its workspace, and may be captured into a graph. The results of a call that returns 64 KB
-or less share one allocation, which lives as long as any of them. Nothing is recorded for autograd: the
+returns and its workspace, and may be captured into a graph. Nothing is recorded for autograd: the
 backward pass is :func:`rms_norm_backward` and :func:`matmul`. Arguments that the kernels cannot
 take raise ``ValueError`` (``TypeError`` for what is no tensor); a missing build raises
 :class:`~tritonk8ssupervisor_amd.ops.NativeUnavailable`.
