@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/EmptyTensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/hip/HIPContextLight.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
@@ -274,6 +275,8 @@ PyObject* matmul(PyObject* const* args, Py_ssize_t nargs) {
     out = &matrix(args[3], "out");
     if (out->size(0) > 1 && out->stride(0) < out->size(1)) wrong_value("the rows of out overlap: it cannot be written to");
     if (out->size(0) != m || out->size(1) != n) wrong_value("out must be (", m, ", ", n, "), not ", shape_of(*out));
+    if (out->requires_grad() && at::GradMode::is_enabled())
+      wrong_value("out requires grad, and nothing is recorded for autograd: write to it under torch.no_grad()");
   }
   if (!out && !THPDtype_Check(args[2])) wrong_type("dtype must be a torch.dtype, not ", Py_TYPE(args[2])->tp_name);
   const ScalarType st = out ? out->scalar_type() : reinterpret_cast<THPDtype*>(args[2])->scalar_type;
@@ -286,6 +289,7 @@ PyObject* matmul(PyObject* const* args, Py_ssize_t nargs) {
   tk8s::fp8_matmul({a.at, b.at, b.by_tile, c.data_ptr(), static_cast<size_t>(m > 1 ? c.stride(0) : n), static_cast<size_t>(m),
                     static_cast<size_t>(n), static_cast<size_t>(k)},
                    *type, dev.stream());
+  if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();  // autograd may have kept what it held
   return THPVariable_Wrap(c);
 }
 

@@ -172,3 +172,12 @@ def test_native_launchers_refuse_before_launching(nat):
             nat.fp8_matmul(far, near, False, 4096, 1 << 20, 1 << 17, 1 << 17, 16, out)
     with pytest.raises(ValueError, match="16-byte"):
         nat.fp8_matmul((4096, 17, 4096, 16), (4096, 16, 4096, 16), False, 4096, 1, 1, 1, 1, 0)
+
+
+def test_matmul_refuses_a_result_that_autograd_would_record(fp8):
+    a, b = _operand(5, 300), _operand(7, 300)
+    leaf = torch.zeros(5, 7, requires_grad=True)
+    with pytest.raises(ValueError, match="requires grad"):
+        fp8.matmul(a, b, out=leaf)
+    with torch.no_grad(), pytest.raises(ValueError, match="run"):
+        fp8.matmul(a, b, out=leaf)

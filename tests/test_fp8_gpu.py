@@ -700,3 +700,22 @@ def test_what_a_call_returns_can_be_resized_and_saved_alone(fp8, cols):
             t.resize_(64, cols).view(torch.uint8).fill_(85)
             for j, u in enumerate(got):
                 assert j <= i or torch.equal(bits_of(u), want[j]), (i, j)
+
+
+@pytest.mark.parametrize("out", TYPES)
+def test_autograd_sees_what_a_product_wrote(fp8, out):
+    a, _ = operand(fp8, 1, 5, 300)
+    b, _ = operand(fp8, 2, 7, 300)
+    c = torch.zeros(5, 7, dtype=out, device="cuda")
+    leaf = torch.ones(5, 7, dtype=out, device="cuda", requires_grad=True)
+    product = leaf * c  # keeps c for its gradient
+    before = c._version
+    fp8.matmul(a, b, out=c)
+    assert c._version == before + 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.no_grad():  # as torch's own calls with out: only what would be recorded is refused
+        assert torch.equal(fp8.matmul(a, b, out=leaf), c)
+    with torch.inference_mode():
+        held = torch.zeros(5, 7, dtype=out, device="cuda")
+        assert torch.equal(fp8.matmul(a, b, out=held), c)

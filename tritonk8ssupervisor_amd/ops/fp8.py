@@ -100,8 +100,8 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
 def matmul(a, b, *, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """``a @ b.T`` of two :class:`Quantized` (or pairs of values and scales): rows of a x rows of b, in
     ``dtype`` (float32, bfloat16 or float16). ``a`` has a scale for each 128 columns of a row, ``b`` the same
-    or one for each 128 x 128. ``out``: a matrix to write to instead of a new one; it must not overlap
-    the operands. At most 2^34 values, rows and columns counted up to a multiple of 64. Scales that do not lie block by block, as :func:`quantize` lays them out, are copied.
+    or one for each 128 x 128. ``out``: a matrix to write to instead of a new one, in its own type whatever
+    ``dtype`` is; it must not overlap the operands, nor require grad where autograd records. At most 2^34 values, rows and columns counted up to a multiple of 64. Scales that do not lie block by block, as :func:`quantize` lays them out, are copied.
 
     A float32 result is exact to 32-bit sums. For the 16-bit types the matrix instruction lines up 8
     products at a time and drops what is below 2^-13 of the largest, which is far below their rounding
