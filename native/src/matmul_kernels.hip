@@ -225,10 +225,10 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 // 16 (4) bytes for each lane from base + offset to LDS at `to` + 16 (4) * lane. Written as assembly
 // so that the compiler does not wait for all of them before it next reads LDS; no register is written.
 __device__ __forceinline__ void load_lds16(unsigned to, const uint8_t* base, unsigned offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "m0", "memory");
 }
 __device__ __forceinline__ void load_lds4(unsigned to, const uint8_t* base, unsigned offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "m0", "memory");
 }
 
 // Waits until at most kLeft of this wave's loads are on their way, then for the other waves.
@@ -592,7 +592,7 @@ constexpr int kSplitPitch = 68;              // floats of a row of partial sums
 
 // A dword for each lane from its own address to LDS.
 __device__ __forceinline__ void load_lds4_each(unsigned to, const uint8_t* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "m0", "memory");
 }
 
 template <class O, bool kExact, int WAVES>
@@ -816,7 +816,7 @@ constexpr int kSmallSlot = 64 * 128 + 256;
 constexpr int kSmallPitch = 36;  // floats of a row of partial sums
 
 __device__ __forceinline__ void load_lds16_each(unsigned to, const uint8_t* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "m0", "memory");
 }
 
 template <class O, bool kExact, int WAVES>

@@ -181,3 +181,18 @@ def test_matmul_refuses_a_result_that_autograd_would_record(fp8):
         fp8.matmul(a, b, out=leaf)
     with torch.no_grad(), pytest.raises(ValueError, match="run"):
         fp8.matmul(a, b, out=leaf)
+
+
+def test_assembly_declares_what_it_writes():
+    """The loads to LDS move their address to m0: the compiler has to know."""
+    import re
+    from pathlib import Path
+
+    sources = Path(__file__).resolve().parents[1] / "native" / "src"
+    found = 0
+    for f in sources.glob("*.hip"):
+        for text in re.findall(r"asm volatile\((.*?)\);", f.read_text(), re.S):
+            if "m0" in text.split(":")[0]:
+                found += 1
+                assert re.search(r':[^:]*"m0"[^:]*$', text), (f.name, text)
+    assert found
