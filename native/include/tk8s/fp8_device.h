@@ -200,10 +200,6 @@ __device__ __forceinline__ float round_tiny_to_odd(double v) {
   return __uint_as_float((odd_bits(v) & 0x80000000u) | whole | (steps != static_cast<double>(whole) ? 1u : 0u));
 }
 
-// Whether v is not 0 and below 2^-126: least <= kTiny for the least of these.
-constexpr unsigned kTiny = 0x38100000u - 2;
-__device__ __forceinline__ unsigned from_zero(double v) { return (odd_bits(v) & 0x7fffffffu) - 1; }
-
 // 1 / sqrt(x) to the last bits of 64: the instruction's first 2^-25 or so, then one step of third order.
 // 0 and infinity keep what the instruction says.
 __device__ __forceinline__ double inverse_sqrt(double x) {

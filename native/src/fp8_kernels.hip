@@ -60,19 +60,20 @@ __device__ __forceinline__ void norm_eight(const NormArgs& a, size_t row, int co
     least = min(least, from_border(y[j]));
     top = max(top, magnitude_bits(y[j]));
   }
-  if (__builtin_amdgcn_ballot_w64(near_border(least) || top < low) != 0 || a.y) {
+  const bool small = top < low;
+  if (__builtin_amdgcn_ballot_w64(near_border(least) || small) != 0 || a.y) {
     Packed8<T> o;
     float y32[8];
-    least = ~0u;
+    unsigned any = 0;
     auto y64 = [&](int j) { return static_cast<double>(unpack(h, j)) * rstd * static_cast<double>(unpack(w, j)); };
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const double v = y64(j);
       y[j] = round_to_odd(v);
       y32[j] = sizeof(T) == 4 ? static_cast<float>(v) : y[j];
-      least = min(least, from_zero(v));
+      any |= odd_bits(v);
     }
-    if (__builtin_amdgcn_ballot_w64(least <= kTiny) != 0) {
+    if (__builtin_amdgcn_ballot_w64(small && any << 1 != 0) != 0) {  // some are not 0, and below 2^-126 perhaps
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         y[j] = round_tiny_to_odd(y64(j));
