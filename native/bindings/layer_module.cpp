@@ -42,7 +42,10 @@ std::string shape_of(const Tensor& t) {
 
 const Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) wrong_type(name, " must be a tensor, not ", Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  if (t.is_neg()) wrong_value(name, " is negated only when it is read: give its resolve_neg()");  // its memory has the other sign
+  if (t._is_zerotensor()) wrong_value(name, " is zeros without memory: give a copy of it");
+  return t;
 }
 
 const Tensor& matrix(PyObject* o, const char* name) {

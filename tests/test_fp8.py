@@ -196,3 +196,22 @@ def test_assembly_declares_what_it_writes():
                 found += 1
                 assert re.search(r':[^:]*"m0"[^:]*$', text), (f.name, text)
     assert found
+
+
+def test_tensors_that_stand_for_other_values_are_refused(fp8):
+    """A lazily negated tensor's memory holds the other sign; zeros may have no memory at all."""
+    z = torch.randn(4, 1, dtype=torch.complex64)
+    x = z.conj().imag  # rows x 1: its one column is contiguous
+    assert x.is_neg()
+    w, r = torch.ones(1), torch.ones(4)
+    for call in (lambda: fp8.quantize(x), lambda: fp8.rms_norm(x, w), lambda: fp8.rms_norm(torch.ones(4, 1), w, residual=x),
+                 lambda: fp8.rms_norm(torch.ones(1, 1), z[0].conj().imag), lambda: fp8.rms_norm_backward(x, torch.ones(4, 1), w, r)):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+    with pytest.raises(ValueError, match="runs on a GPU"):
+        fp8.quantize(x.resolve_neg())
+    zeros = torch._efficientzerotensor((4, 1))  # a tangent that autograd never wrote down
+    for call in (lambda: fp8.quantize(zeros), lambda: fp8.rms_norm(torch.ones(4, 1), w, residual=zeros),
+                 lambda: fp8.rms_norm_backward(torch.ones(4, 1), torch.ones(4, 1), w, r, dh=zeros)):
+        with pytest.raises(ValueError, match="without memory"):
+            call()
