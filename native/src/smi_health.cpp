@@ -44,7 +44,7 @@ const char* link_name(amdsmi_link_type_t t) {
 }
 
 // Collects the metrics one GPU supports; a metric the platform does not expose is simply
-// absent (listed under "unsupported") rather than an error.
+// absent (a temperature: null), listed under "unsupported", rather than an error.
 std::string gpu_json(amdsmi_processor_handle h, int index) {
   Json j;
   std::vector<std::string> unsupported;
@@ -62,8 +62,7 @@ std::string gpu_json(amdsmi_processor_handle h, int index) {
   if (amdsmi_get_gpu_driver_info(h, &drv) == AMDSMI_STATUS_SUCCESS)
     j.kv("driver", std::string(drv.driver_name) + " " + std::string(drv.driver_version));
 
-  Json temps;
-  bool any_temp = false;
+  Json temps;  // every sensor: null where the platform has no reading
   const std::pair<const char*, amdsmi_temperature_type_t> sensors[] = {
       {"edge", AMDSMI_TEMPERATURE_TYPE_EDGE},
       {"hotspot", AMDSMI_TEMPERATURE_TYPE_HOTSPOT},
@@ -72,12 +71,12 @@ std::string gpu_json(amdsmi_processor_handle h, int index) {
     int64_t c = 0;
     if (amdsmi_get_temp_metric(h, type, AMDSMI_TEMP_CURRENT, &c) == AMDSMI_STATUS_SUCCESS) {
       temps.kv(name, static_cast<int64_t>(c));
-      any_temp = true;
     } else {
+      temps.raw(name, "null");
       unsupported.push_back(std::string("temp_") + name);
     }
   }
-  if (any_temp) j.raw("temp_c", temps.str());
+  j.raw("temp_c", temps.str());
 
   amdsmi_power_info_t pw{};
   if (amdsmi_get_power_info(h, &pw) == AMDSMI_STATUS_SUCCESS) {

@@ -197,3 +197,33 @@ def test_pci_bus_id_from_kfd_location():
     from tritonk8ssupervisor_amd.models.hostinfo import HostGpu
 
     assert HostGpu(ordinal=0, location_id=(0xa4 << 8) | (1 << 3) | 2, domain=1).pci_bus_id == "0001:a4:01.2"
+
+
+def test_a_platform_without_temperatures_reports_none(monkeypatch, capsys):
+    """AMD SMI of some virtual machines reads no temperature: the sensors are there, without a value, and nothing
+    that shows or sums them takes that for a number."""
+    from types import SimpleNamespace
+
+    from tritonk8ssupervisor_amd.agent import agent
+    from tritonk8ssupervisor_amd.cli import kubectl, main
+    from tritonk8ssupervisor_amd.ops import fakesmi
+
+    monkeypatch.setenv("TK8S_FAKE_GPUS", "2")
+    report = fakesmi.report(2)
+    for g in report["gpus"]:
+        g["temp_c"] = {"edge": None, "hotspot": None, "vram": None}
+    plugin = DevicePlugin([0, 1], inventory=fake_inventory(2))
+    plugin.update_from_smi(report)
+    ann = plugin.telemetry_annotations()
+    assert "amd.com/gpu-temp-hotspot-max-c" not in ann and ann["amd.com/gpu-power-w"] == str(180 + 181)
+    devices = [{"id": d.id, "health": d.health, "telemetry": d.telemetry} for d in plugin.devices_]
+    assert "hotspot" not in kubectl._device_line(devices[0]) and "power=180W" in kubectl._device_line(devices[0])
+    node = {"metadata": {"name": "n1"}, "status": {"devices": devices, "allocatable": {}}}
+    assert "None" not in kubectl.fmt_top([node], []) and "361W" in kubectl.fmt_top([node], [])
+    report["gpus"][1]["temp_c"]["hotspot"] = 47
+    monkeypatch.setattr(agent, "read_smi", lambda: report)
+    assert main.cmd_gpu_health(SimpleNamespace(json=False)) == 0
+    out = capsys.readouterr().out
+    assert "47C" in out and "None" not in out and "-C" not in out
+    plugin.update_from_smi(report)
+    assert plugin.telemetry_annotations()["amd.com/gpu-temp-hotspot-max-c"] == "47"

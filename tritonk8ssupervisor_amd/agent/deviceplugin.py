@@ -135,7 +135,7 @@ class DevicePlugin:
         tel = [d.telemetry for d in self.devices_ if d.telemetry]
         if not tel:
             return {}
-        hot = [t["temp_c"]["hotspot"] for t in tel if "hotspot" in t.get("temp_c", {})]
+        hot = [c for t in tel if (c := (t.get("temp_c") or {}).get("hotspot")) is not None]
         watts = [t["power"]["current_w"] for t in tel if "current_w" in t.get("power", {})]
         ue = sum(int(t.get("ecc", {}).get("uncorrectable", 0) or 0) for t in tel)
         out = {"amd.com/gpu-health-source": "amdsmi", "amd.com/gpu-ecc-uncorrectable": str(ue)}

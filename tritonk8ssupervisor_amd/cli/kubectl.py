@@ -634,7 +634,7 @@ def fmt_top(nodes: list[dict], pods: list[dict], usage: dict | None = None) -> s
     rows = [["NAME", "CPU(cores)", "MEMORY(bytes)", "GPU(USED/ALLOC)", "HOTSPOT-MAX", "POWER", "VRAM-USED"]]
     for n in nodes:
         tel = [d.get("telemetry") or {} for d in n["status"].get("devices", [])]
-        hot = [t["temp_c"]["hotspot"] for t in tel if "hotspot" in t.get("temp_c", {})]
+        hot = [c for t in tel if (c := (t.get("temp_c") or {}).get("hotspot")) is not None]
         watts = [t["power"]["current_w"] for t in tel if "current_w" in t.get("power", {})]
         vram = [t["vram_used_bytes"] for t in tel if "vram_used_bytes" in t]
         name = n["metadata"]["name"]

@@ -232,9 +232,9 @@ def cmd_gpu_health(args) -> int:
         print(f"{'GPU':<4} {'PCI':<13} {'HEALTHY':<8} {'HOTSPOT':>7} {'POWER':>6} {'VRAM USED':>10} {'ECC UE/CE':>10}")
         for g in r.get("gpus", []):
             ecc = g.get("ecc", {})
-            used = g.get("vram_used_bytes")
+            used, hot = g.get("vram_used_bytes"), (g.get("temp_c") or {}).get("hotspot")
             print(f"{g.get('index', '?'):<4} {g.get('pci_bus_id', '?'):<13} {str(g.get('healthy')):<8} "
-                  f"{str(g.get('temp_c', {}).get('hotspot', '-')) + 'C':>7} "
+                  f"{(f'{hot}C' if hot is not None else '-'):>7} "
                   f"{str(g.get('power', {}).get('current_w', '-')) + 'W':>6} "
                   f"{(f'{used / 2**30:.1f}GiB' if used is not None else '-'):>10} "
                   f"{str(ecc.get('uncorrectable', '-')) + '/' + str(ecc.get('correctable', '-')):>10}")

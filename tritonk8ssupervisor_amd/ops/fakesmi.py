@@ -41,7 +41,7 @@ def report(n: int | None = None, with_links: bool = True) -> dict:
         bad = ue.get(i, 0)
         gpus.append({
             "index": i, "pci_bus_id": f"0000:{0x10 + i:02x}:00.0", "market_name": "AMD Instinct MI355 OAM (fake)",
-            "cu_count": 256, "oam_id": i, "temp_c": {"hotspot": 40 + i, "vram": 33},
+            "cu_count": 256, "oam_id": i, "temp_c": {"edge": None, "hotspot": 40 + i, "vram": 33},
             "power": {"current_w": 180 + i, "limit_w": 1400}, "vram_total_bytes": 309220868096,
             "vram_used_bytes": 297766912, "ecc": {"correctable": 0, "uncorrectable": bad, "deferred": 0},
             "activity": {"gfx_pct": 0, "umc_pct": 0}, "healthy": bad == 0, "unsupported": ["temp_edge"],
