@@ -113,3 +113,24 @@ def test_the_norms_weight_gradient_is_held_to_its_sum(nat, rows):
         assert nat.layer_weight_sum_error(np.float32(planted), dy, h, rstd) > 1, planted
     with pytest.raises(ValueError):
         nat.layer_weight_sum_error(0.0, dy, h, rstd[:-1])
+
+
+def test_a_machines_share_of_the_host_burnin_is_judged_by_its_layer_too():
+    """A GPU whose matrix cores failed does not pass for a bad link from another machine's GPU."""
+    from tritonk8ssupervisor_amd.burnin import split_host_result
+
+    def device(i, layer_ok, digest_ok=True, link_ok=True):
+        fine = {"ok": True}
+        return {"device": i, "ok": layer_ok and digest_ok, "hbm": fine, "md5": fine, "digest_ok": True, "copy": fine,
+                "layer": {"ok": layer_ok, "digest": "d"}, "layer_digest_ok": digest_ok,
+                "peers": [{"ok": link_ok, "src_device": 1 - i, "dst_device": i}]}
+
+    def share(**kw):
+        return split_host_result({"ok": True, "layer_expected": "d", "devices": [device(0, **kw), device(1, True)]}, [4, 5], [4], {"pulls": []})
+
+    for link_ok in (True, False):
+        good = share(layer_ok=True, link_ok=link_ok)
+        assert good["layer"]["digest"] == good["layer_expected"] == "d"
+        assert not share(layer_ok=False, link_ok=link_ok)["ok"]
+        assert not share(layer_ok=True, digest_ok=False, link_ok=link_ok)["ok"]
+    assert share(layer_ok=True, digest_ok="unpinned")["ok"]

@@ -89,11 +89,12 @@ def split_host_result(result: dict, burnin_gpus: list[int], machine_gpus: list[i
         d = devs.get(pos[g])
         if d is None:
             return None
-        # The machine is judged on its own GPUs: their HBM/MD5/copy checks and the xGMI pulls
+        # The machine is judged on its own GPUs: their HBM/MD5/copy/layer checks and the xGMI pulls
         # between them. Pulls from other machines' GPUs are the fabric's business (the RCCL Job
         # validates it cluster-wide once every node is Ready); they are kept for the record.
         peers = [p for p in d.get("peers") or [] if p.get("src_device") in mine]
-        own = all((d.get(k) or {}).get("ok", True) for k in ("hbm", "md5", "copy")) and d.get("digest_ok", True)
+        own = all((d.get(k) or {}).get("ok", True) for k in ("hbm", "md5", "copy", "layer")) and \
+            d.get("digest_ok", True) and d.get("layer_digest_ok", True)
         foreign_bad = any(not p.get("ok") for p in d.get("peers") or [] if p.get("src_device") not in mine)
         ok = bool(d.get("ok")) or bool(foreign_bad and own and all(p.get("ok") for p in peers) and "error" not in d)
         sub_devs.append({**d, "device": i, "host_index": g, "ok": ok, "peers": peers,
@@ -108,11 +109,12 @@ def split_host_result(result: dict, burnin_gpus: list[int], machine_gpus: list[i
            "timings_ms": result.get("timings_ms", {}),
            "gpuinfo": {**{k: v for k, v in info.items() if k not in ("devices", "links")}, "device_count": len(sub_info),
                        "devices": sub_info, "links": sub_links}}
-    for key in ("hbm", "md5", "copy"):
+    for key in ("hbm", "md5", "copy", "layer"):
         if key in first:
             out[key] = first[key]
-    if "md5_expected" in result:
-        out["md5_expected"] = result["md5_expected"]
+    for key in ("md5_expected", "layer_expected"):
+        if key in result:
+            out[key] = result[key]
     if report is None and any(d.get("peers") for d in result.get("devices", [])):
         from .xgmi import link_report
 
