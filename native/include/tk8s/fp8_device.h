@@ -71,7 +71,7 @@ template <class T> __device__ __forceinline__ void at_any(T* p, const Packed8<T>
 
 // n = 1..7 of them. kParts (16-bit values only): in parts of 4, 2 and 1, three loads (stores) where one for each
 // value would be seven in a row's last lane, which the others wait for (gradients of 5475 x 438: 15.6 ->
-// 13.2 us; 32-bit values are better off with seven: a norm of 1031 x 5003 takes 22.9 us, 27.3 in parts).
+// 13.2 us; 32-bit values are better off with seven: parts made a norm of 1031 x 5003 19 % slower).
 template <int kDwords> struct __attribute__((packed, aligned(2))) Dwords2 { unsigned d[kDwords]; };
 
 template <bool kParts, class T> __device__ __forceinline__ Packed8<T> load_tail(const T* p, int n) {

@@ -95,8 +95,9 @@ struct Fp8Matrix {
 
 // h = x + residual, rounded to the type (no residual: h = x, nothing is stored);
 // rstd = 1 / sqrt(mean(h^2) + eps); y = h * rstd * weight. q/scales: y in 8 bits with a scale for
-// each 128 columns of a row; y itself and rstd are stored where their pointers are given. Every
-// sum and y are in 64 bits and rounded once. A block that holds a NaN or an infinity is NaN.
+// each 128 columns of a row; y itself and rstd are stored where their pointers are given. Sums and rstd are in 64
+// bits; y and its 8-bit values are those of y in 64 bits, rounded once (it is computed in 32 where that gives the same 8
+// bits). y beyond the range of 32 bits is an infinity. A block that holds a NaN or an infinity is NaN.
 struct NormArgs {
   const void* x;
   size_t ldx;

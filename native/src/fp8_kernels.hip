@@ -117,8 +117,9 @@ template <class T> __device__ __forceinline__ double add_squares(const Packed8<T
 // neighbouring lanes hold exactly one block of 128. The sum of squares and rstd are in 64 bits. A block
 // walks rows a grid apart: the weight stays in its registers, and the next row is requested before the
 // sum of this one is waited for. kWhole: rows are a whole number of chunks. 16384 x 8192, 16-bit, with a
-// residual: 163 us, 5.8 TB/s, which HBM bounds; 1031 x 5003 without: 9.2 us, 1.7 TB/s, four rows for a CU
-// one after the other; one row of 4096: 3.3 us, the latency of its loads and of its sum.
+// residual: 163 us, 5.8 TB/s, which HBM bounds; 1031 x 5003 without: 9.1 us, 1.7 TB/s, the time of a row and, for
+// seven of the 1024 blocks, which are all there at once, of a second one (in 32 bits 11.4, from HBM, where 512 blocks
+// make a third pass for seven rows); one row of 4096: 3.3 us, the latency of its loads and of its sum.
 template <class T, class W, int TPR, int NCH, bool kWhole>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(NormArgs a) {
   constexpr int kRows = TPR < 256 ? 256 / TPR : 1;

@@ -1,11 +1,11 @@
 #!/usr/bin/env bash
-# Where the RCCL communicator start goes with the unpacked library (utils/rccl_unpack.py): one
+# Where the RCCL communicator start goes with the operator's own build (utils/rccl_unpack.py): one
 # tk8s-rccl run at n=1 with RCCL's INFO log timestamped to the microsecond.
 set -o pipefail
 out=gpurun_out/${1:-r5_rccl_init}
 mkdir -p $out
 lib=$(python3 -c "from tritonk8ssupervisor_amd.utils.rccl_unpack import library_dir; print(library_dir() or '')")
-[ -n "$lib" ] || { echo "no unpacked RCCL (run build first)"; exit 1; }
+[ -n "$lib" ] || { echo "no RCCL built from source is kept (python3 -m tritonk8ssupervisor_amd.utils.rccl_unpack /path/to/librccl.so.1)"; exit 1; }
 for i in 1 2; do
   LD_LIBRARY_PATH=$lib NCCL_DEBUG=INFO NCCL_DEBUG_SUBSYS=ALL NCCL_DEBUG_TIMESTAMP_LEVELS=ALL \
     NCCL_DEBUG_TIMESTAMP_FORMAT="%H:%M:%S.%6f " TK8S_TRACE=1 \

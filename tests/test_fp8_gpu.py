@@ -719,3 +719,18 @@ def test_autograd_sees_what_a_product_wrote(fp8, out):
     with torch.inference_mode():
         held = torch.zeros(5, 7, dtype=out, device="cuda")
         assert torch.equal(fp8.matmul(a, b, out=held), c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_beyond_32_bits(fp8, dtype):
+    """A y of 5e39 is an infinity, and its block NaN; the row's other blocks are what they are."""
+    x, w = torch.zeros(2, 300, dtype=dtype), torch.full((300,), 3e38, dtype=dtype)
+    x[0, 5], x[1, 200] = 1, -1
+    for normed in (False, True):
+        n = fp8.rms_norm(x.cuda(), w.cuda(), eps=0.0, normed=normed)
+        s, q = bits(n.scales), host(n.values)
+        assert s.tolist() == [[255, 127, 127], [127, 255, 127]]
+        assert np.isnan(q[0, :128]).all() and np.isnan(q[1, 128:256]).all() and np.isnan(q).sum() == 256
+        assert (q[~np.isnan(q)] == 0).all()
+    y = host(n.y)
+    assert y[0, 5] == np.inf and y[1, 200] == -np.inf and np.count_nonzero(y) == 2

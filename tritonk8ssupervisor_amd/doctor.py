@@ -68,8 +68,8 @@ def common_checks() -> list[dict]:
 
 def transparent_huge_pages(path: str = "/sys/kernel/mm/transparent_hugepage/enabled") -> dict:
     """The fabric rank's malloc goes on huge pages when the kernel allows it (madvise or always:
-    HIP's copies of RCCL's 108 MB code object, 318 -> 202 ms of the communicator start,
-    profiles/r5_thp/); with ``never`` the advice is ignored and the rank runs as before."""
+    HIP's copies of RCCL's code while it loads, 318 -> 202 ms of the communicator start with
+    a library for gfx950 alone, profiles/r5_thp/); with ``never`` the advice is ignored and the rank runs as before."""
     try:
         text = Path(path).read_text()
     except OSError as e:

@@ -34,10 +34,10 @@ def rccl_rank_env(fake: bool = False) -> tuple[list[dict], Path | None]:
     fail-fast knobs and the ``rccl.*`` fault points are passed on here; with real GPUs the rank
     loads the operator's own RCCL build for this GPU where one is kept (utils/rccl_unpack.py: no
     inflation of every target's code in its communicator start) and runs glibc's malloc on transparent
-    huge pages: HIP copies RCCL's 108 MB code object several times while loading it (its stream
-    read, comgr's set_data, ...), each copy into freshly faulted 4 KiB pages -- ~190 ms of a
-    285 ms load was memcpy; on huge pages (the kernel's madvise mode is enough) the communicator
-    start went from 318 to 202 ms on the MI355X (profiles/r5_thp/); the rank then loads that code
+    huge pages: HIP copies RCCL's code several times while loading it, each copy into freshly
+    faulted 4 KiB pages -- ~190 ms of a 285 ms load was memcpy with a library for gfx950 alone;
+    on huge pages (the kernel's madvise mode is enough) its communicator start went from 318 to
+    202 ms on the MI355X (profiles/r5_thp/); the rank then loads that code
     and makes its stream on threads while the unique id is made (profiles/r6_rccl_prewarm/).
     Off-switches: TK8S_RCCL_UNPACKED=0, TK8S_RCCL_THP=0, TK8S_RCCL_PREWARM=0.
 
